@@ -488,6 +488,43 @@ int sgta_stem_level0_x3(const float* img, long img_bs, const float* hm, long hm_
 int sgta_dcnv2_x3(const float* x, long x_bs, const float* om, long om_bs, const void* wt, long wt_bytes, const float* bias,
                   float* y, long y_bs, int B, int Cin, int H, int W, int Cout, int mt, int log_tw, int act, sgta_stream_t stream);
 
+/* ---- attention over sequences of any length (attn_fwd.hip, attn_bwd.hip) ----------------------------------------------------
+ * One softmax map with a learned relative position bias by buckets (sgta_rel_attn_*):
+ *   o[b,i,h] = sum_j softmax_j( scale q[b,i,h].k[b,j,h'] + w[lut[clamp(j - p_i, -reach, reach) + reach], h] ) v[b,j,h']
+ * or two maps whose difference is taken with a learned weight (sgta_diff_attn_*):
+ *   o = ( softmax(scale q1.k1) - lambda softmax(scale q2.k2) ) v,   lambda = exp(w0.w1) - exp(w2.w3) + lam_init
+ * with p_i = q_start[b] + i and h' = h / (H / Hkv).  Keys j < kv_len[b] are seen, under ``causal`` those with j <= p_i; queries
+ * i < q_len[b] are computed, rows behind them are left as they are, and nothing behind kv_len / q_len is read.  A query that
+ * sees no key has an output and gradients of zero.  Next to sgta_mhca_fwd_f32: any lengths, shared key / value heads, 16-bit
+ * types, gradients.
+ *
+ * All pointers to device memory; type of q, k, v, w, out, out2 and of all gradients: dtype 0 f32, 1 IEEE half, 2 bfloat16.
+ * Strides in elements {batch, position, head, map}; the last dimension is contiguous; strides whole 16 bytes, pointers 16-byte
+ * aligned.  D, Dv multiples of 8; one map: D = Dv <= 128; two maps: D <= 64, Dv <= 128.  H % Hkv == 0.  q_len / kv_len /
+ * q_start int32 [B] or NULL (Lq, Lk, 0).  w: table [num_buckets, H] or the four vectors [4, D], contiguous.
+ * lut: int32 [2 reach + 1], bucket of each distance; from ``reach`` on (<= 1024) it stays the same.
+ * stats: f32 [maps][B][H][Lq][2] (reference and log2 of the sum, for the backward pass) or NULL.
+ * out2: [B, Lq, H, Dv] contiguous, the second map's product with v (for the backward pass) or NULL.
+ * ws: f32 workspace of sgta_attn_fwd_ws_floats() floats (0: not used), written before it is read; calls that may
+ * overlap take one each. */
+typedef struct {
+  const void *q, *k, *v, *w;
+  void *out, *out2;
+  float* stats;
+  const void* dout;
+  void *dq, *dk, *dv, *dw;
+  long sq[4], sk[4], sv[4], so[4], sdo[4], sdq[4], sdk[4], sdv[4];
+  const int *q_len, *kv_len, *q_start, *lut;
+  float* ws;
+  long ws_floats;
+  int B, Lq, Lk, H, Hkv, D, Dv, causal, dtype, reach, num_buckets;
+  float scale, lam_init;
+} sgta_attn_t;
+
+long sgta_attn_fwd_ws_floats(const sgta_attn_t* a, int maps);
+int sgta_rel_attn_fwd(const sgta_attn_t* a, sgta_stream_t stream);
+int sgta_diff_attn_fwd(const sgta_attn_t* a, sgta_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,6 +13,18 @@ _i = ctypes.c_int
 _l = ctypes.c_long
 _f = ctypes.c_float
 
+
+class AttnArgs(ctypes.Structure):
+    """sgta_attn_t: the arguments of the sgta_rel_attn_* / sgta_diff_attn_* entry points."""
+    _fields_ = ([(n, _p) for n in ("q", "k", "v", "w", "out", "out2", "stats", "dout", "dq", "dk", "dv", "dw")]
+                + [(n, _l * 4) for n in ("sq", "sk", "sv", "so", "sdo", "sdq", "sdk", "sdv")]
+                + [(n, _p) for n in ("q_len", "kv_len", "q_start", "lut", "ws")] + [("ws_floats", _l)]
+                + [(n, _i) for n in ("B", "Lq", "Lk", "H", "Hkv", "D", "Dv", "causal", "dtype", "reach", "num_buckets")]
+                + [("scale", _f), ("lam_init", _f)])
+
+
+_attn = ctypes.POINTER(AttnArgs)
+
 # name -> argtypes (return type is always int); must mirror include/sgta_hip.h
 SIGNATURES = {
     "sgta_version": [],
@@ -81,6 +93,10 @@ SIGNATURES = {
     "sgta_pnp_batched": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _p],
     "sgta_gn_refine": [_p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _p],
     "sgta_softargmax": [_p, _p, _i, _i, _i, _i, _f, _f, _p],
+    # attention over sequences of any length: learned relative position bias by buckets; difference of two maps
+    "sgta_attn_fwd_ws_floats": [_attn, _i],
+    "sgta_rel_attn_fwd": [_attn, _p],
+    "sgta_diff_attn_fwd": [_attn, _p],
 }
 
 _lib = None
@@ -103,7 +119,7 @@ def load():
     for name, argtypes in SIGNATURES.items():
         fn = getattr(lib, name)          # AttributeError = header / library out of sync: loud
         fn.argtypes = argtypes
-        fn.restype = ctypes.c_long if name.endswith("_max_elems") else ctypes.c_int
+        fn.restype = ctypes.c_long if name.endswith(("_max_elems", "_ws_floats")) else ctypes.c_int
     _lib = lib
     return lib
 

@@ -1,0 +1,210 @@
+// What the attention kernels share (attn_fwd.hip, attn_bwd.hip): element types, LDS tiles and their fragments, staging.
+//
+// Every product runs on 32x32 matrix tiles: v_mfma_f32_32x32x16_{f16,bf16}, or eight v_mfma_f32_32x32x2_f32 for float, whose
+// operands hold the same (row, 8 k) fragment per lane: lane l has row l & 31 and k = 8 (l >> 5) + 0..7 of a step of 16 (for
+// float, instruction e multiplies element e of both halves: any pairing of k is right as long as both operands use it).
+// A result has its column on the lane (l & 31) and row 8 (r >> 2) + 4 (l >> 5) + (r & 3) in register r.  Eight consecutive
+// result registers are therefore an operand fragment of 16 rows in the order {0-3, 8-11} / {4-7, 12-15} of the two lane
+// halves; read_cols() hands out the other operand in that same order, so softmax weights go from one product into the next
+// without leaving their registers.
+#pragma once
+#include "common.h"
+#include "../../include/sgta_hip.h"
+
+typedef sgta_attn_t AttnArgs;
+
+#define LOG2E 1.4426950408889634f
+#define LN2 0.6931471805599453f
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+enum { TY_F32 = 0, TY_F16 = 1, TY_BF16 = 2 };
+
+template <int TY> struct El;
+template <> struct El<TY_F32> {
+  typedef float T;
+  typedef f32x8 Frag;
+  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+  }
+  static __device__ __forceinline__ Frag frag(f32x8 v) { return v; }
+  static __device__ __forceinline__ float load(const T* p) { return *p; }
+  static __device__ __forceinline__ void store4(T* p, f32x4 v) { *reinterpret_cast<f32x4*>(p) = v; }
+  static __device__ __forceinline__ void store(T* p, float v) { *p = v; }
+};
+template <bool F16> struct El16 {
+  typedef typename H16<F16>::T T;
+  typedef typename H16<F16>::x8 Frag;
+  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) { return H16<F16>::mfma32(a, b, c); }
+  // IEEE half: values beyond 65504 are clamped, as everywhere in the 16-bit data path
+  static __device__ __forceinline__ Frag frag(f32x8 v) { return H16<F16>::cvt8(v); }
+  static __device__ __forceinline__ float load(const T* p) { return (float)*p; }
+  static __device__ __forceinline__ void store4(T* p, f32x4 v) { *reinterpret_cast<typename H16<F16>::x4*>(p) = H16<F16>::cvt4(v); }
+  static __device__ __forceinline__ void store(T* p, float v) {
+    f32x4 t = {v, 0.0f, 0.0f, 0.0f};
+    *p = H16<F16>::cvt4(t)[0];
+  }
+};
+template <> struct El<TY_F16> : El16<true> {};
+template <> struct El<TY_BF16> : El16<false> {};
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// the other lane half's value beside one's own: {value of lane l & 31, value of lane 32 + (l & 31)}
+__device__ __forceinline__ void both_halves(float x, float& lo, float& hi) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  lo = __uint_as_float(r[0]);
+  hi = __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float half_sum(float x) {
+  float a, b;
+  both_halves(x, a, b);
+  return a + b;
+}
+__device__ __forceinline__ float half_max(float x) {
+  float a, b;
+  both_halves(x, a, b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+  return x;
+}
+
+// One operand tile in LDS: rows of COLS elements in 16-byte pieces, XOR-swizzled by the row so that the 8 rows which one
+// quarter of a wave reads at a time fall on different banks.
+template <int TY, int COLS> struct Tile {
+  typedef typename El<TY>::T T;
+  typedef typename El<TY>::Frag Frag;
+  static constexpr int SZ = sizeof(T);
+  static constexpr int ROWB = COLS * SZ;              // bytes per row: 64 ... 512
+  static constexpr int CH = ROWB / 16;                // pieces per row
+  static constexpr int EPC = 16 / SZ;                 // elements per piece
+  static __device__ __forceinline__ int swz(int row) { return ROWB >= 128 ? (row & 7) : ((row >> 1) & 3); }
+  static __device__ __forceinline__ int piece(int row, int ch) { return row * ROWB + ((ch ^ swz(row)) << 4); }
+
+  // operand fragment of row ``row``: elements 16 s + 8 half + 0..7
+  static __device__ __forceinline__ Frag read_rows(const char* lds, int row, int s, int half) {
+    if constexpr (TY == TY_F32) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(lds + piece(row, 4 * s + 2 * half));
+      const f32x4 b = *reinterpret_cast<const f32x4*>(lds + piece(row, 4 * s + 2 * half + 1));
+      return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+      return *reinterpret_cast<const Frag*>(lds + piece(row, 2 * s + half));
+    }
+  }
+  // operand fragment of COLUMN 32 blk + (lane & 31): rows row0 + {0-3, 8-11} + 4 half, the order of the result registers
+  static __device__ __forceinline__ Frag read_cols(const char* lds, int row0, int blk, int lane) {
+    if constexpr (TY == TY_F32) {
+      const int col = 32 * blk + (lane & 31), half = lane >> 5;
+      Frag f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int row = row0 + 4 * half + (e & 3) + 8 * (e >> 2);
+        f[e] = *reinterpret_cast<const float*>(lds + piece(row, col >> 2) + (col & 3) * 4);
+      }
+      return f;
+    } else {
+      // transposing read: each 16 lanes fetch 4 rows x 16 columns, lane i of them gets column i of the 4 rows
+      const int g = lane >> 4, i = lane & 15;
+      const int row = row0 + 4 * (g >> 1) + (i >> 2), col = 32 * blk + 16 * (g & 1) + 4 * (i & 3);
+      typedef __attribute__((address_space(3))) s16x4* lp;
+      s16x8 v;
+      const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(lds + piece(row, col >> 3) + (col & 4) * 2));
+      const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(lds + piece(row + 8, col >> 3) + (col & 4) * 2));
+      v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+      return __builtin_bit_cast(Frag, v);
+    }
+  }
+};
+
+// Rows [row0, row0 + ROWS) of a strided matrix on their way into a Tile: global loads into registers now, LDS stores later.
+// Rows from ``rows`` on and elements from ``cols`` on are zero and never read: what lies there may be anything.
+template <int TY, int COLS, int ROWS, int NT> struct Stage {
+  typedef Tile<TY, COLS> Tl;
+  typedef typename El<TY>::T T;
+  static constexpr int N = ROWS * Tl::CH / NT;
+  static_assert(ROWS * Tl::CH % NT == 0, "whole pieces per thread");
+  u32x4 r[N];
+  __device__ __forceinline__ void load(const T* p, long ld, int row0, int rows, int cols, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = tid + i * NT, row = row0 + c / Tl::CH, e = (c % Tl::CH) * Tl::EPC;
+      u32x4 z = {0, 0, 0, 0};
+      r[i] = z;
+      if (row < rows && e < cols) r[i] = *reinterpret_cast<const u32x4*>(p + (long)row * ld + e);
+    }
+  }
+  __device__ __forceinline__ void store(char* lds, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = tid + i * NT;
+      *reinterpret_cast<u32x4*>(lds + Tl::piece(c / Tl::CH, c % Tl::CH)) = r[i];
+    }
+  }
+};
+
+// eight consecutive elements of a global row as an operand fragment (zero where ``ok`` is false)
+template <int TY> __device__ __forceinline__ typename El<TY>::Frag global_frag(const typename El<TY>::T* p, bool ok) {
+  typename El<TY>::Frag f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = 0;
+  if (ok) f = *reinterpret_cast<const typename El<TY>::Frag*>(p);
+  return f;
+}
+
+// lambda = exp(w0 . w1) - exp(w2 . w3) + init, by one wave; e1, e2: the two exponentials
+template <int TY> __device__ __forceinline__ float diff_lambda(const AttnArgs& a, float& e1, float& e2) {
+  const typename El<TY>::T* w = (const typename El<TY>::T*)a.w;
+  const int lane = threadIdx.x & 63;
+  float s1 = 0.0f, s2 = 0.0f;
+  for (int d = lane; d < a.D; d += 64) {
+    s1 = fmaf(El<TY>::load(w + d), El<TY>::load(w + a.D + d), s1);
+    s2 = fmaf(El<TY>::load(w + 2 * a.D + d), El<TY>::load(w + 3 * a.D + d), s2);
+  }
+  e1 = expf(wave_sum(s1));
+  e2 = expf(wave_sum(s2));
+  return e1 - e2 + a.lam_init;
+}
+
+__device__ __forceinline__ int clamp_len(const int* len, int b, int most) { return len ? min(max(len[b], 0), most) : most; }
+// positions are held in 32 bits: lengths are below 2^29, and a start beyond +- 2^30 sees the same keys at the same (farthest)
+// buckets as one there
+__device__ __forceinline__ int start_of(const int* start, int b) { return start ? min(max(start[b], -(1 << 30)), 1 << 30) : 0; }
+
+// The bias of head h over distances, in LDS: entry [rel + reach + BIAS_PAD] for |rel| <= reach + BIAS_PAD, in units of log2;
+// from ``reach`` on the bucket stays the same.  A tile that comes within ``reach`` of its queries' positions indexes it
+// without a clamp: its distances go at most BIAS_PAD further.
+#define BIAS_PAD 128
+__device__ __forceinline__ int bias_size(int reach) { return 2 * (reach + BIAS_PAD) + 1; }
+template <int TY> __device__ __forceinline__ float bias_log2(const AttnArgs& a, int rel, int h) {
+  const int at = min(max(rel, -a.reach), a.reach) + a.reach;
+  const float t = El<TY>::load((const typename El<TY>::T*)a.w + (long)a.lut[at] * a.H + h);
+  // a type's lowest value stays finite (a row that has nothing else keeps equal weights), an infinity stays one
+  const float s = t * LOG2E;
+  return (fabsf(s) == INFINITY && fabsf(t) != INFINITY) ? copysignf(3.402823466e38f, s) : s;
+}
+template <int TY> __device__ __forceinline__ void fill_bias(const AttnArgs& a, float* tab, int h, int tid, int nt) {
+  const int n = bias_size(a.reach);
+  for (int i = tid; i < n; i += nt) tab[i] = bias_log2<TY>(a, i - a.reach - BIAS_PAD, h);
+}
+// beyond this a bias absorbs the scores it is added to: such tiles add it to each score instead of folding it into the exponent
+#define BIAS_FOLD 1e30f
+
+// lets a kernel use up to 160 KB of LDS on the current device (once a device), refuses more
+template <auto KERNEL> static int allow_lds(int bytes) {
+  static bool done[SGTA_MAX_DEVICES];
+  if (bytes > 160 * 1024) return SGTA_EBADARG;
+  const int slot = sgta_device_slot();
+  if (!done[slot]) {
+    const hipError_t e = hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    if (e != hipSuccess) return (int)e;
+    done[slot] = true;
+  }
+  return SGTA_OK;
+}

@@ -1,0 +1,355 @@
+"""Attention with a bucketed relative bias and differential attention (sgtapose_amd/ops_attn.py) against the formulas in 64 bits.
+
+Tolerances are bounds, element by element, from the arithmetic of the kernels (u = eps / 2 of the element type, e = 2^-24):
+  scores    D products summed in f32, times the scale, plus the bias, minus the reference: off by at most
+            es = e ((D + 3) scale sum|q||k| + 4 |s| + 16), so a weight is off by a factor exp(2 es) (its own score and the sum's)
+  weights   rounded to the element type before the product with v: u of each (IEEE half: 2^-25 at least, where it is subnormal)
+  sums      Lk terms in f32: e Lk of the sum of magnitudes
+  output    rounded once more: u |o|
+"""
+import math
+
+import pytest
+import torch
+
+from sgtapose_amd import ops_attn
+from sgtapose_amd._lib import SgtaHipError
+
+gpu = pytest.mark.gpu
+E = 2.0 ** -24
+U = {torch.float32: 0.0, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+FLUSH = {torch.float32: 0.0, torch.float16: 2.0 ** -25, torch.bfloat16: 0.0}
+ALL = [torch.float32, torch.float16, torch.bfloat16]
+NAMES = {torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16"}
+
+
+# ---- the formulas, in 64 bits -----------------------------------------------------------------
+def bucket_of(d, n, far, both):
+    at = 0
+    if both:
+        n //= 2
+        at, d = (n if d > 0 else 0), abs(d)
+    else:
+        d = max(-d, 0)
+    if d < n // 2:
+        return at + d
+    return at + min(n - 1, n // 2 + math.floor(math.log(d / (n // 2)) / math.log(far / (n // 2)) * (n - n // 2) + 1e-9))
+
+
+class Case:
+    """Inputs of one call and everything a bound needs, in float64 on the CPU."""
+
+    def __init__(self, maps, dtype, B, Lq, Lk, H, Hkv, D, Dv=None, causal=False, q_len=None, kv_len=None, q_start=None, buckets=32, far=40,
+                 seed=0, scale=None, dout_scale=1.0):
+        g = torch.Generator().manual_seed(seed)
+        Dv = D if Dv is None else Dv
+        mp = (2,) if maps == 2 else ()
+        rn = lambda *s: torch.randn(*s, generator=g)                                              # noqa: E731
+        self.maps, self.dtype, self.causal, self.buckets, self.far = maps, dtype, causal, buckets, far
+        self.dims = (B, Lq, Lk, H, Hkv, D, Dv)
+        self.q, self.k, self.v = rn(B, Lq, H, *mp, D).to(dtype), rn(B, Lk, Hkv, *mp, D).to(dtype), rn(B, Lk, Hkv, Dv).to(dtype)
+        self.w = (rn(buckets, H) if maps == 1 else 0.3 * rn(4, D)).to(dtype)
+        self.dout = (dout_scale * rn(B, Lq, H, Dv)).to(dtype)
+        self.lens = dict(q_len=q_len, kv_len=kv_len, q_start=q_start)
+        self.scale = scale
+
+    def kwargs(self, dev):
+        kw = {n: None if t is None else torch.tensor(t, dtype=torch.int32, device=dev) for n, t in self.lens.items()}
+        kw.update(causal=self.causal, scale=self.scale)
+        if self.maps == 1:
+            kw.update(max_distance=self.far, bidirectional=not self.causal)
+        return kw
+
+    def reference(self):
+        """-> dict of float64 results and bounds."""
+        B, Lq, Lk, H, Hkv, D, Dv = self.dims
+        G, T = H // Hkv, self.dtype
+        f = lambda t: t.double()                                                                  # noqa: E731
+        nq = torch.tensor(self.lens["q_len"] or [Lq] * B).clamp(0, Lq)
+        nk = torch.tensor(self.lens["kv_len"] or [Lk] * B).clamp(0, Lk)
+        st = torch.tensor(self.lens["q_start"] or [0] * B)
+        i, j = torch.arange(Lq), torch.arange(Lk)
+        rel = j[None, None] - i[None, :, None] - st[:, None, None]
+        seen = (j[None, None] < nk[:, None, None]) & (i[None, :, None] < nq[:, None, None])
+        if self.causal:
+            seen = seen & (rel <= 0)
+        seen = seen[:, None]
+        # what lies behind the lengths takes no part, whatever it is
+        q, k, v, do = (torch.where((torch.arange(t.shape[1])[None] < n[:, None]).reshape(B, -1, *[1] * (t.dim() - 2)), f(t), 0.0)
+                       for t, n in ((self.q, nq), (self.k, nk), (self.v, nk), (self.dout, nq)))
+        q, do = q.transpose(1, 2), do.transpose(1, 2)
+        k, v = k.transpose(1, 2).repeat_interleave(G, 1), v.transpose(1, 2).repeat_interleave(G, 1)
+        c = D ** -0.5 if self.scale is None else self.scale
+        bias = 0.0
+        if self.maps == 1:
+            rel = rel.clamp(-self.far, self.far)                    # the buckets stay the same from there on
+            lo, hi = int(rel.min()), int(rel.max())
+            of = torch.tensor([bucket_of(d, self.buckets, self.far, not self.causal) for d in range(lo, hi + 1)])[rel - lo]
+            bias = f(self.w)[of].permute(0, 3, 1, 2)
+        P, es, qs, ks, mags = [], [], [], [], []
+        for p in range(self.maps):
+            qp, kp = (q, k) if self.maps == 1 else (q[:, :, :, p], k[:, :, :, p])
+            s = c * (qp @ kp.transpose(-1, -2)) + bias
+            mag = c * (qp.abs() @ kp.abs().transpose(-1, -2))
+            es.append(E * ((D + 3) * mag + 4 * s.abs().clamp(max=1e4) + 16).amax((-1, -2), keepdim=True))
+            s = torch.where(seen, s, -math.inf)
+            m = s.amax(-1, keepdim=True)
+            e = torch.exp(s - torch.where(m == -math.inf, 0.0, m))
+            t = e.sum(-1, keepdim=True)
+            P.append(e / torch.where(t == 0, 1.0, t))
+            qs.append(qp)
+            ks.append(kp)
+        u, tiny, sums = U[T], FLUSH[T], Lk * E
+        lam, lam_err = 0.0, 0.0
+        if self.maps == 2:
+            w = f(self.w)
+            e1, e2 = torch.exp((w[0] * w[1]).sum()), torch.exp((w[2] * w[3]).sum())
+            lam = e1 - e2 + 0.8
+            lam_err = float(E * (D + 8) * (e1 * (1 + (w[0] * w[1]).abs().sum()) + e2 * (1 + (w[2] * w[3]).abs().sum()) + 2))
+        sgn = (1.0, -lam)
+        o = sum(sgn[p] * (P[p] @ v) for p in range(self.maps))
+        va = v.abs()
+        o_mid = sum(abs(sgn[p]) * ((u + 2 * es[p] + sums) * (P[p] @ va) + tiny * (seen.double() @ va)) for p in range(self.maps))
+        if self.maps == 2:
+            o_mid = o_mid + lam_err * (P[1] @ va)
+        r = dict(out=o.transpose(1, 2), out_tol=(o_mid * 1.01 + u * o.abs() + 4 * E * o.abs() + 1e-30).transpose(1, 2), nq=nq, nk=nk, P=P)
+        self.parts = dict(q=qs, k=ks, v=v, do=do, P=P, es=es, c=c, seen=seen, lam=lam, o_mid=o_mid, u=u, tiny=tiny, sums=sums,
+                          of=of if self.maps == 1 else None, st=st, nq=nq, nk=nk)
+        return r
+
+
+def within(name, got, want, tol, rows=None):
+    d = (got.double().cpu() - want).abs()
+    if rows is not None:
+        keep = torch.arange(got.shape[1])[None] < rows[:, None]
+        d, tol = d[keep], tol.expand(want.shape)[keep]
+    bad = ~(d <= tol)
+    assert not bad.any(), "%s: %d of %d beyond the bound, worst %.3g against %.3g" % (
+        name, int(bad.sum()), bad.numel(), float(d[bad].max()), float(tol.expand(d.shape)[bad].min()))
+
+
+def forward(c, dev="cuda", **more):
+    fn = ops_attn.rel_attention if c.maps == 1 else ops_attn.diff_attention
+    return fn(c.q.to(dev), c.k.to(dev), c.v.to(dev), c.w.to(dev), **c.kwargs(dev), **more)
+
+
+def check_forward(c):
+    r = c.reference()
+    got = forward(c)
+    torch.cuda.synchronize()
+    within("out", got, r["out"], r["out_tol"], r["nq"])
+    return got
+
+
+# ---- host ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("n,far,both", [(32, 128, True), (32, 128, False), (16, 64, True), (64, 200, False), (4, 5, True), (2, 2, False),
+                                        (6, 1024, True)])
+def test_buckets_follow_the_definition(n, far, both):
+    if both and n // 2 < 2:
+        pytest.skip("one bucket a direction")
+    got = ops_attn.relative_buckets(n, far, both)
+    reach = ops_attn.bucket_reach(n, far, both)
+    assert len(got) == 2 * reach + 1
+    assert got == [bucket_of(d, n, far, both) for d in range(-reach, reach + 1)]
+    assert bucket_of(-far - 7, n, far, both) == got[0] and bucket_of(far + 7, n, far, both) == got[-1]
+
+
+def _cpu(maps=1, B=2, Lq=5, Lk=7, H=4, Hkv=2, D=16, Dv=None, dtype=torch.bfloat16):
+    mp = (2,) if maps == 2 else ()
+    z = lambda *s: torch.zeros(*s, dtype=dtype)                                                   # noqa: E731
+    return [z(B, Lq, H, *mp, D), z(B, Lk, Hkv, *mp, D), z(B, Lk, Hkv, Dv or D), z(32, H) if maps == 1 else z(4, D)]
+
+
+@pytest.mark.parametrize("what,change", [
+    ("heads not shared evenly", dict(H=4, Hkv=3)), ("head size not a multiple of 8", dict(D=12)), ("head size too large", dict(D=136)),
+    ("no keys", dict(Lk=0)), ("a type that has no kernel", dict(dtype=torch.float64)), ("different head sizes", dict(D=16, Dv=32))])
+def test_rel_attention_refuses_shapes(what, change):
+    with pytest.raises(SgtaHipError):
+        ops_attn.rel_attention(*_cpu(**change))
+
+
+@pytest.mark.parametrize("change", [dict(D=72), dict(D=64, Dv=136), dict(Hkv=3), dict(Lq=0), dict(D=20)])
+def test_diff_attention_refuses_shapes(change):
+    with pytest.raises(SgtaHipError):
+        ops_attn.diff_attention(*_cpu(2, **change))
+
+
+def test_refuses_what_is_not_on_the_gpu_and_bad_operands():
+    for maps, fn in ((1, ops_attn.rel_attention), (2, ops_attn.diff_attention)):
+        q, k, v, w = _cpu(maps)
+        with pytest.raises(SgtaHipError, match="GPU"):
+            fn(q, k, v, w)
+        with pytest.raises(SgtaHipError):
+            fn(q, k.float(), v, w)
+        with pytest.raises(SgtaHipError):
+            fn(q, k, v[:1], w)
+        with pytest.raises(SgtaHipError):
+            fn(q, k, v, w[:, :-1])
+        with pytest.raises(SgtaHipError, match="contiguous"):
+            fn(q.transpose(-1, -2).contiguous().transpose(-1, -2), k, v, w)
+        with pytest.raises(SgtaHipError, match="kv_len"):
+            fn(q, k, v, w, kv_len=torch.zeros(2, dtype=torch.int64))
+        for bad in (0.0, -1.0, math.inf, math.nan):
+            with pytest.raises(SgtaHipError, match="scale"):
+                fn(q, k, v, w, scale=bad)
+    q, k, v, w = _cpu()
+    for kw in (dict(max_distance=8), dict(max_distance=2000), dict(bidirectional=False, max_distance=16)):
+        with pytest.raises(SgtaHipError, match="max_distance"):
+            ops_attn.rel_attention(q, k, v, w, **kw)
+    with pytest.raises(SgtaHipError, match="buckets"):
+        ops_attn.rel_attention(q, k, v, w[:3])
+
+
+def test_c_entries_refuse_before_they_launch():
+    import ctypes
+    from sgtapose_amd import _lib
+    lib = _lib.load()
+    ok = dict(q=64, k=64, v=64, w=64, out=64, lut=64, B=1, Lq=4, Lk=4, H=2, Hkv=2, D=16, Dv=16, dtype=2, reach=8, num_buckets=8, scale=0.25)
+    for change in (dict(q=None), dict(q=65), dict(H=3), dict(D=12), dict(Dv=24), dict(dtype=3), dict(scale=0.0), dict(reach=0), dict(reach=1025),
+                   dict(lut=None), dict(Lk=0), dict(sq=(ctypes.c_long * 4)(16, 4, 16, 0)), dict(Lq=1 << 29), dict(out=None)):
+        a = _lib.AttnArgs(**{**ok, **change})
+        assert lib.sgta_rel_attn_fwd(ctypes.byref(a), None) < 0, change
+        assert lib.sgta_attn_fwd_ws_floats(ctypes.byref(a), 1) == 0
+    assert lib.sgta_rel_attn_fwd(None, None) < 0 and lib.sgta_diff_attn_fwd(None, None) < 0
+    a = _lib.AttnArgs(**{**ok, "Lk": 1 << 20})                        # parts of the keys need a workspace
+    assert lib.sgta_attn_fwd_ws_floats(ctypes.byref(a), 1) > 0 and lib.sgta_rel_attn_fwd(ctypes.byref(a), None) < 0
+
+
+# ---- forward --------------------------------------------------------------------------------------
+SHAPES = [(1, 1, 1, 1, 1), (2, 1, 33, 2, 1), (1, 5, 64, 4, 4), (2, 33, 129, 4, 2), (1, 128, 128, 2, 2), (2, 129, 65, 3, 1), (1, 300, 517, 2, 1)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ALL, ids=NAMES.get)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_rel_forward(dtype, causal, shape):
+    B, Lq, Lk, H, Hkv = shape
+    for D in (16, 64, 128):
+        check_forward(Case(1, dtype, B, Lq, Lk, H, Hkv, D, causal=causal, seed=D, q_start=[max(0, Lk - Lq)] * B if causal else None))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ALL, ids=NAMES.get)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_diff_forward(dtype, causal, shape):
+    B, Lq, Lk, H, Hkv = shape
+    for D, Dv in ((16, 32), (64, 128), (40, 24)):
+        check_forward(Case(2, dtype, B, Lq, Lk, H, Hkv, D, Dv, causal=causal, seed=D, q_start=[max(0, Lk - Lq)] * B if causal else None))
+
+
+@gpu
+@pytest.mark.parametrize("D", [8, 24, 32, 40, 96, 104])
+def test_rel_forward_head_sizes(D):
+    for dtype in ALL:
+        check_forward(Case(1, dtype, 2, 70, 90, 2, 2, D, seed=D))
+        check_forward(Case(1, dtype, 2, 2, 90, 4, 2, D, seed=D))
+
+
+@gpu
+@pytest.mark.parametrize("maps", [1, 2])
+@pytest.mark.parametrize("Lq", [1, 3, 150])
+def test_lengths_and_starts(maps, Lq):
+    """Empty sequences, one key, all keys; starts before the first key (a causal query that sees nothing) and past the last;
+    whatever lies behind the lengths (here NaN) takes no part, output rows behind the queries stay as they are."""
+    for causal in (False, True):
+        c = Case(maps, torch.bfloat16, 6, Lq, 200, 4, 2, 32, causal=causal, kv_len=[0, 1, 200, 77, 128, 500], seed=Lq,
+                 q_len=[Lq, Lq, 0, max(1, Lq // 2), Lq, Lq + 9], q_start=[0, 0, 3, 76, -5, 2 ** 30 + 5])
+        r = c.reference()
+        for b in range(6):
+            c.k[b, min(200, c.lens["kv_len"][b]):] = math.nan
+            c.v[b, min(200, c.lens["kv_len"][b]):] = math.nan
+            c.q[b, min(Lq, c.lens["q_len"][b]):] = math.nan
+        out = torch.full((6, Lq, 4, 32), 7.0, dtype=torch.bfloat16, device="cuda")
+        forward(c, out=out)
+        within("out", out, r["out"], r["out_tol"], r["nq"])
+        behind = torch.arange(Lq)[None] >= r["nq"][:, None]
+        assert bool((out.cpu()[behind] == 7.0).all())
+        assert bool((out[0].cpu()[: int(r["nq"][0])] == 0).all())
+        fresh = forward(c)
+        assert bool((fresh.cpu()[behind] == 0).all()) and torch.equal(fresh.cpu()[~behind], out.cpu()[~behind])
+
+
+@gpu
+@pytest.mark.parametrize("maps", [1, 2])
+@pytest.mark.parametrize("dtype", ALL, ids=NAMES.get)
+def test_few_queries_against_long_caches(maps, dtype):
+    """The split over the keys: lengths around the parts' ends, several rows a head, shared heads."""
+    for Lq, H, Hkv, Lk in ((1, 8, 2, 2500), (4, 8, 1, 1025), (1, 1, 1, 5000), (8, 4, 1, 513)):
+        n = [Lk, Lk - 1, 129]
+        check_forward(Case(maps, dtype, 3, Lq, Lk, H, Hkv, 64, 64 if maps == 1 else 128, causal=True, kv_len=n, q_start=[x - Lq for x in n], seed=Lq))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ALL, ids=NAMES.get)
+@pytest.mark.parametrize("Lq,Lk", [(1, 300), (200, 300)])
+def test_rel_table_infinities_and_lowest_values(dtype, Lq, Lk):
+    """-inf hides a bucket's keys, the type's lowest value weighs nothing beside others and evenly among its like."""
+    for causal in (False, True):
+        for value in (-math.inf, torch.finfo(dtype).min):
+            c = Case(1, dtype, 1, Lq, Lk, 2, 2, 32, causal=causal, q_start=[Lk - Lq] if causal else None)
+            c.w[::2] = value
+            check_forward(c)
+            if value == -math.inf:
+                c.w[:] = value                                       # every row is empty: zeros
+                assert bool((forward(c) == 0).all())
+        c = Case(1, dtype, 1, Lq, Lk, 2, 2, 32, causal=causal, q_start=[Lk - Lq] if causal else None)
+        c.w[:] = torch.finfo(dtype).min                              # all buckets at the lowest value: equal weights
+        check_forward(c)
+
+
+@gpu
+def test_strided_operands_and_output():
+    """Slices of one projection, a cache in another order, an output inside a wider buffer."""
+    for maps in (1, 2):
+        for Lq in (2, 150):
+            c = Case(maps, torch.float16, 2, Lq, 150, 4, 2, 32, seed=5)
+            r = c.reference()
+            mp = (2,) if maps == 2 else ()
+            wide = torch.randn(2, Lq, 4, 3, *mp, 32, device="cuda").half()
+            q = wide[:, :, :, 1]
+            q.copy_(c.q)
+            k = c.k.cuda().transpose(1, 2).contiguous().transpose(1, 2)                   # [B, heads, L, D] in memory
+            v = c.v.cuda().permute(1, 0, 2, 3).contiguous().permute(1, 0, 2, 3)           # [L, B, heads, D]
+            buf = torch.full((2, Lq, 4, 64), 5.0, device="cuda").half()
+            fn = ops_attn.rel_attention if maps == 1 else ops_attn.diff_attention
+            fn(q, k, v, c.w.cuda(), buf[..., 32:], **c.kwargs("cuda"))
+            within("out", buf[..., 32:].contiguous(), r["out"], r["out_tol"])
+            assert bool((buf[..., :32] == 5).all())
+            one = c.k[:1].cuda().expand(2, -1, *[-1] * (c.k.dim() - 2))                   # one cache for both samples
+            got = fn(c.q.cuda(), one, c.v.cuda(), c.w.cuda(), **c.kwargs("cuda"))
+            c.k[1] = c.k[0]
+            r = c.reference()
+            within("out", got, r["out"], r["out_tol"])
+            with pytest.raises(SgtaHipError, match="share memory"):
+                fn(q, k, v, c.w.cuda(), buf[:1, ..., 32:].expand(2, -1, -1, -1), **c.kwargs("cuda"))
+
+
+@gpu
+def test_streams_and_graphs():
+    """On a stream that is not the current device's default, and captured: every replay gives what the eager call gives."""
+    for maps in (1, 2):
+        for Lq, Lk in ((1, 1500), (140, 200)):
+            c = Case(maps, torch.bfloat16, 2, Lq, Lk, 4, 2, 64, seed=9)
+            t = [x.cuda() for x in (c.q, c.k, c.v, c.w)]
+            kw = c.kwargs("cuda")
+            fn = ops_attn.rel_attention if maps == 1 else ops_attn.diff_attention
+            want = fn(*t, **kw)
+            s = torch.cuda.Stream()
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                other = fn(*t, **kw)
+            s.synchronize()
+            assert torch.equal(other, want)
+            out = torch.empty_like(want)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                fn(*t, out, **kw)
+            for n in range(3):
+                t[0].copy_(c.q * (n + 1))
+                want = fn(*t, **kw)
+                out.zero_()
+                g.replay()
+                torch.cuda.synchronize()
+                assert torch.equal(out, want)
