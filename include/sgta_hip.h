@@ -525,6 +525,17 @@ long sgta_attn_fwd_ws_floats(const sgta_attn_t* a, int maps);
 int sgta_rel_attn_fwd(const sgta_attn_t* a, sgta_stream_t stream);
 int sgta_diff_attn_fwd(const sgta_attn_t* a, sgta_stream_t stream);
 
+/* ---- token products in 8-bit integers (linear_i8.hip) --------------------------------------------------------------------------
+ * sgta_quant_rows_i8: xs[m] = max|x[m,:]| / 127 (f32), xq[m,k] = x[m,k] / xs[m] rounded to the nearest, ties to even; a row of
+ * zeros has scale and bytes of zero; a row with a not-a-number or an infinity has that as its scale.  x: [M, K] rows of ldx
+ * elements of ``dtype`` (0 f32, 1 IEEE half, 2 bfloat16), any alignment of the rows.
+ * sgta_linear_i8: out[m,n] = relu?( (sum_k xq[m,k] wq[n,k]) xs[m] ws[n] + bias[n] ); the sum is exact.  xq [M, K], wq [N, K]
+ * int8 rows of ldx / ldw bytes; xs f32 [M], ws f32 [N]; bias [N] or NULL and out [M, N] (rows of ldo elements) of ``dtype``.
+ * K <= 131071 and ldx, ldw <= 2^22, else SGTA_ETOOBIG.  Next to sgta_linear_f32. */
+int sgta_quant_rows_i8(const void* x, long ldx, int dtype, signed char* xq, long ldq, float* xs, int M, int K, sgta_stream_t stream);
+int sgta_linear_i8(const signed char* xq, long ldx, const float* xs, const signed char* wq, long ldw, const float* ws,
+                   const void* bias, void* out, long ldo, int M, int N, int K, int relu, int dtype, sgta_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
