@@ -525,6 +525,13 @@ long sgta_attn_fwd_ws_floats(const sgta_attn_t* a, int maps);
 int sgta_rel_attn_fwd(const sgta_attn_t* a, sgta_stream_t stream);
 int sgta_diff_attn_fwd(const sgta_attn_t* a, sgta_stream_t stream);
 
+/* Gradients: dq, dk, dv (strides sdq, sdk, sdv) and dw (w's shape, contiguous; the whole of it) from dout, the forward's operands,
+ * its out, stats (and out2).  Rows behind q_len (dq) and kv_len (dk, dv) are left as they are.  ws: sgta_attn_bwd_ws_floats()
+ * floats.  No atomics in global memory: the same inputs give the same bits. */
+long sgta_attn_bwd_ws_floats(const sgta_attn_t* a, int maps);
+int sgta_rel_attn_bwd(const sgta_attn_t* a, sgta_stream_t stream);
+int sgta_diff_attn_bwd(const sgta_attn_t* a, sgta_stream_t stream);
+
 /* ---- token products in 8-bit integers (linear_i8.hip) --------------------------------------------------------------------------
  * sgta_quant_rows_i8: xs[m] = max|x[m,:]| / 127 (f32), xq[m,k] = x[m,k] / xs[m] rounded to the nearest, ties to even; a row of
  * zeros has scale and bytes of zero; a row with a not-a-number or an infinity has that as its scale.  x: [M, K] rows of ldx

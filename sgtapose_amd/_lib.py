@@ -97,6 +97,9 @@ SIGNATURES = {
     "sgta_attn_fwd_ws_floats": [_attn, _i],
     "sgta_rel_attn_fwd": [_attn, _p],
     "sgta_diff_attn_fwd": [_attn, _p],
+    "sgta_attn_bwd_ws_floats": [_attn, _i],
+    "sgta_rel_attn_bwd": [_attn, _p],
+    "sgta_diff_attn_bwd": [_attn, _p],
     # token products in 8-bit integers
     "sgta_quant_rows_i8": [_p, _l, _i, _p, _l, _p, _i, _i, _p],
     "sgta_linear_i8": [_p, _l, _p, _p, _l, _p, _p, _p, _l, _i, _i, _i, _i, _i, _p],

@@ -1,0 +1,627 @@
+// Gradients of the attention in attn_fwd.hip, from the saved row statistics (reference m and log2 of the sum, so that
+// P = exp2((s - m) - log2 sum) needs no second softmax):
+//   X = dO V^T, delta = rowsum(dO o O), dS = P o (X - delta), dQ = scale dS K, dK = scale dS^T Q, dV = P^T dO,
+//   dtable[b, h] = sum of dS over the pairs in bucket b.
+// Two maps share X:  dS1 = P1 o (X - d1), dS2 = -lambda P2 o (X - d2), d_p = rowsum(dO o O_p), dV = (P1 - lambda P2)^T dO,
+//   dlambda = - sum of d2.
+//
+// No atomics and no Lq x Lk array: every sum has one owner and a fixed order.
+//   attn_dq_kernel   a wave owns 32 queries and walks the keys: delta, dQ, the table's gradient by distance
+//   attn_dkv_kernel  a wave owns 32 keys and walks the queries of all heads that share them: dK, dV
+//   *_dw_kernel      sums the work-groups' parts of the learned weights' gradient
+// The price is that scores and X are computed twice (7 products instead of 5); what it buys is that gradients are the same from
+// run to run and that dQ (f32, Lq x D a head and key block) is never read back.
+//
+// IEEE half: dS is rounded to half as the operand of the next product.  Gradients arrive at any magnitude, so it is first scaled
+// by a power of two that brings the largest |dO| of the row (dQ) or of all queries of the shared heads (dK) next to one.
+#include "attn_common.h"
+
+int attn_check(const AttnArgs* a, int maps);
+
+__device__ __forceinline__ float pow2_to_one(float top) {          // 2^-exponent(top), 1 for zero and for what is not finite
+  const int e = (__float_as_uint(top) >> 23) & 255;
+  return (e == 0 || e == 255) ? 1.0f : __uint_as_float((unsigned)(min(max(254 - e, 1), 254)) << 23);
+}
+
+// the workspace, in floats
+struct BwdWork {
+  long delta, part, top;       // [maps][B][H][Lq]; per (b, h, query block): sums by distance, or of d2; largest |dO|
+  long total;
+  int nblk, nrel;
+  __host__ __device__ BwdWork(const AttnArgs& a, int maps) {
+    nblk = (a.Lq + 127) / 128;
+    nrel = maps == 1 ? 2 * (a.reach + BIAS_PAD) + 1 : 1;
+    const long blocks = (long)a.B * a.H * nblk;
+    delta = 0;
+    part = (long)maps * a.B * a.H * a.Lq;
+    top = part + blocks * nrel;
+    total = top + blocks;
+  }
+};
+
+template <int TY, int MAPS, int DQ, int DV, bool BIAS>
+__global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
+  typedef typename El<TY>::T T;
+  typedef typename El<TY>::Frag Frag;
+  constexpr int KT = TY == TY_F32 ? 32 : 64;
+  typedef Tile<TY, DQ> TK;
+  typedef Tile<TY, DV> TV;
+  constexpr int KB = MAPS * KT * TK::ROWB, VB = KT * TV::ROWB;
+  extern __shared__ __align__(16) char smem[];       // 2 x (K maps, V) | bias table | 4 waves x 2 lane halves of sums by distance
+  const BwdWork wk(a, MAPS);
+  float* tab = reinterpret_cast<float*>(smem + 2 * (KB + VB));
+  float* hist = tab + wk.nrel;
+  __shared__ float red[4];
+  const int nblk = wk.nblk, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
+  const int bh = blockIdx.x % (a.B * a.H), b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
+  const int blk = a.causal ? nblk - 1 - blockIdx.x / (a.B * a.H) : blockIdx.x / (a.B * a.H);
+  const int nq = clamp_len(a.q_len, b, a.Lq), nk = clamp_len(a.kv_len, b, a.Lk), st = start_of(a.q_start, b);
+  const int blk0 = blk * 128;
+  float* part = a.ws + wk.part + ((long)bh * nblk + blk) * wk.nrel;
+  float* topw = a.ws + wk.top + (long)bh * nblk + blk;
+  if (blk0 >= nq) {
+    for (int i = tid; i < wk.nrel; i += 256) part[i] = 0.0f;
+    if (tid == 0) *topw = 0.0f;
+    return;
+  }
+  const int row0 = blk0 + wave * 32, row = row0 + li;
+  const bool ok = row < nq;
+  float lam = 0.0f;
+  if constexpr (MAPS == 2) {
+    float e1, e2;
+    lam = diff_lambda<TY>(a, e1, e2);
+  }
+
+  // the row's operands, delta and largest |dO|
+  Frag q[MAPS][DQ / 16], g[DV / 16];
+  float m[MAPS], lg[MAPS], dl[MAPS], top = 0.0f;
+  {
+    const T* qp = (const T*)a.q + b * a.sq[0] + row * a.sq[1] + h * a.sq[2];
+#pragma unroll
+    for (int p = 0; p < MAPS; ++p)
+#pragma unroll
+      for (int s = 0; s < DQ / 16; ++s) {
+        const int d = 16 * s + 8 * half;
+        q[p][s] = global_frag<TY>(qp + (MAPS == 2 ? p * a.sq[3] : 0) + d, ok && d < a.D);
+      }
+    const T* gp = (const T*)a.dout + b * a.sdo[0] + row * a.sdo[1] + h * a.sdo[2];
+    const T* op = (const T*)a.out + b * a.so[0] + row * a.so[1] + h * a.so[2];
+    const T* o2 = MAPS == 2 ? (const T*)a.out2 + (((long)b * a.Lq + row) * a.H + h) * a.Dv : op;
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int s = 0; s < DV / 16; ++s) {
+      const int d = 16 * s + 8 * half;
+      const bool in = ok && d < a.Dv;
+      g[s] = global_frag<TY>(gp + d, in);
+      const Frag o = global_frag<TY>(op + d, in);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        s1 = fmaf((float)g[s][e], (float)o[e], s1);
+        top = fmaxf(top, fabsf((float)g[s][e]));
+      }
+      if constexpr (MAPS == 2) {
+        const Frag y = global_frag<TY>(o2 + d, in);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s2 = fmaf((float)g[s][e], (float)y[e], s2);
+      }
+    }
+    s1 = half_sum(s1);
+    top = half_max(top);
+    if constexpr (MAPS == 2) {
+      s2 = half_sum(s2);
+      dl[0] = fmaf(lam, s2, s1);
+      dl[1] = s2;
+    } else {
+      dl[0] = s1;
+    }
+#pragma unroll
+    for (int p = 0; p < MAPS; ++p) {
+      const long at = (((long)p * a.B + b) * a.H + h) * a.Lq + row;
+      m[p] = ok ? a.stats[2 * at] : 0.0f;
+      lg[p] = ok ? a.stats[2 * at + 1] : INFINITY;
+      if (ok && half == 0) a.ws[wk.delta + at] = dl[p];
+    }
+    float t = top;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) t = fmaxf(t, __shfl_xor(t, d));
+    if (lane == 0) red[wave] = t;
+    __syncthreads();
+    if (tid == 0) *topw = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    if constexpr (MAPS == 2) {
+      __syncthreads();
+      float t2 = half == 0 && ok ? dl[1] : 0.0f;
+      t2 = wave_sum(t2);
+      if (lane == 0) red[wave] = t2;
+      __syncthreads();
+      if (tid == 0) part[0] = (red[0] + red[1]) + (red[2] + red[3]);
+    }
+  }
+  const float rs = TY == TY_F16 ? pow2_to_one(top) : 1.0f;          // power of two for dS
+  const float irs = 1.0f / rs;
+
+  const int pos = st + row, pmin = st + row0, pmax = st + row0 + 31;
+  const int limit = ok ? min(nk - 1, a.causal ? pos : nk - 1) : -1;
+  float far_l = 0.0f, far_r = 0.0f, sum_l = 0.0f, sum_r = 0.0f;
+  bool fold = true;
+  const float* tb = tab;
+  float* mine = hist;
+  if constexpr (BIAS) {
+    fill_bias<TY>(a, tab, h, tid, 256);
+    for (int i = tid; i < 8 * wk.nrel; i += 256) hist[i] = 0.0f;
+    far_l = bias_log2<TY>(a, -a.reach, h);
+    far_r = bias_log2<TY>(a, a.reach, h);
+    fold = fabsf(far_l) < BIAS_FOLD && fabsf(far_r) < BIAS_FOLD;
+    tb = tab + a.reach + BIAS_PAD;
+    mine = hist + (2 * wave + half) * wk.nrel + a.reach + BIAS_PAD;
+  }
+  const float c2 = a.scale * LOG2E;
+  const int last_row = min(blk0 + 127, nq - 1);
+  const int seen = a.causal ? min(nk, max(st + last_row + 1, 0)) : nk;
+  const int nt = (seen + KT - 1) / KT;
+  const int wave_last = a.causal ? min(seen - 1, st + min(row0 + 31, nq - 1)) : seen - 1;
+  const bool active = row0 < nq;
+
+  f32x16 dq[MAPS][DQ / 32];
+#pragma unroll
+  for (int p = 0; p < MAPS; ++p)
+#pragma unroll
+    for (int d = 0; d < DQ / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dq[p][d][r] = 0.0f;
+
+  const T* kp = (const T*)a.k + b * a.sk[0] + hk * a.sk[2];
+  const T* vp = (const T*)a.v + b * a.sv[0] + hk * a.sv[2];
+  Stage<TY, DQ, KT, 256> ks[MAPS];
+  Stage<TY, DV, KT, 256> vs;
+  auto fetch = [&](int j0) {
+#pragma unroll
+    for (int p = 0; p < MAPS; ++p) ks[p].load(kp + (MAPS == 2 ? p * a.sk[3] : 0), a.sk[1], j0, seen, a.D, tid);
+    vs.load(vp, a.sv[1], j0, seen, a.Dv, tid);
+  };
+  auto put = [&](int buf) {
+    char* base = smem + buf * (KB + VB);
+#pragma unroll
+    for (int p = 0; p < MAPS; ++p) ks[p].store(base + p * KT * TK::ROWB, tid);
+    vs.store(base + KB, tid);
+  };
+  if (nt > 0) {
+    fetch(0);
+    put(0);
+  }
+  __syncthreads();
+  for (int t = 0; t < nt; ++t) {
+    const char* kt = smem + (t & 1) * (KB + VB);
+    const char* vt = kt + KB;
+    if (t + 1 < nt) fetch((t + 1) * KT);
+#pragma unroll
+    for (int u = 0; u < KT / 32; ++u) {
+      const int j0 = t * KT + 32 * u;
+      if (!active || j0 > wave_last) continue;
+      f32x16 x;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < DV / 16; ++k) x = El<TY>::mma(TV::read_rows(vt, 32 * u + li, k, half), g[k], x);
+      const bool masked = __any(limit < j0 + 31);
+      const int last = limit - j0 - 4 * half;
+#pragma unroll
+      for (int p = 0; p < MAPS; ++p) {
+        f32x16 s;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < DQ / 16; ++k) s = El<TY>::mma(TK::read_rows(kt + p * KT * TK::ROWB, 32 * u + li, k, half), q[p][k], s);
+        float cc = c2, add = -m[p] - lg[p];
+        bool left = false, right = false;
+        if constexpr (BIAS) {
+          left = j0 + 31 - pmin <= -a.reach;
+          right = j0 - pmax >= a.reach;
+          if ((left || right) && fold) {
+            add = ((left ? far_l : far_r) - m[p]) - lg[p];
+          } else {
+            const float* tp = tb + (j0 + 4 * half - pos);
+            cc = 1.0f;
+            add = -lg[p];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const float bias = left ? far_l : right ? far_r : tp[8 * (r >> 2) + (r & 3)];
+              s[r] = fmaf(s[r], c2, bias) - m[p];
+            }
+          }
+        }
+        if (masked) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + (r & 3) <= last ? s[r] : -INFINITY;
+        }
+        const float nd = -dl[p] * rs, sg = (MAPS == 2 && p == 1) ? -lam : 1.0f;
+        float tot[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          f32x8 ds;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            float w = exp2_(fmaf(s[8 * k + r], cc, add));
+            if (MAPS == 2 && p == 1) w *= sg;
+            ds[r] = w * fmaf(x[8 * k + r], rs, nd);
+            if (BIAS) {
+              tot[r & 3] += ds[r];
+              s[8 * k + r] = ds[r];
+            }
+          }
+          const Frag f = El<TY>::frag(ds);
+#pragma unroll
+          for (int d = 0; d < DQ / 32; ++d)
+            dq[p][d] = El<TY>::mma(TK::read_cols(kt + p * KT * TK::ROWB, 32 * u + 16 * k, d, lane), f, dq[p][d]);
+        }
+        if constexpr (BIAS) {
+          if (left || right) {
+            const float all = ((tot[0] + tot[1]) + (tot[2] + tot[3])) * irs;
+            if (left) sum_l += all; else sum_r += all;
+          } else {
+            // one distance a lane and instruction, the lane halves apart: no two lanes add to one place
+            float* hp = mine + (j0 + 4 * half - pos);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) __hip_atomic_fetch_add(hp + 8 * (r >> 2) + (r & 3), s[r] * irs, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+          }
+        }
+      }
+    }
+    if (t + 1 < nt) put((t & 1) ^ 1);
+    __syncthreads();
+  }
+
+  if (ok) {
+    T* o = (T*)a.dq + b * a.sdq[0] + row * a.sdq[1] + h * a.sdq[2];
+    const float f = a.scale * irs;
+#pragma unroll
+    for (int p = 0; p < MAPS; ++p)
+#pragma unroll
+      for (int d = 0; d < DQ / 32; ++d)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int col = 32 * d + 8 * c + 4 * half;
+          f32x4 y = {dq[p][d][4 * c] * f, dq[p][d][4 * c + 1] * f, dq[p][d][4 * c + 2] * f, dq[p][d][4 * c + 3] * f};
+          if (col < a.D) El<TY>::store4(o + (MAPS == 2 ? p * a.sdq[3] : 0) + col, y);
+        }
+  }
+  if constexpr (BIAS) {
+    sum_l = wave_sum(sum_l);
+    sum_r = wave_sum(sum_r);
+    if (lane == 0) {                                  // the ends of the table stand for everything beyond
+      hist[2 * wave * wk.nrel] += sum_l;
+      hist[2 * wave * wk.nrel + wk.nrel - 1] += sum_r;
+    }
+    __syncthreads();
+    for (int i = tid; i < wk.nrel; i += 256) {
+      float v = 0.0f;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) v += hist[c * wk.nrel + i];
+      part[i] = v;
+    }
+  }
+}
+
+template <int TY, int MAPS, int DQ, int DV, bool BIAS>
+__global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnArgs a, int nblk) {
+  typedef typename El<TY>::T T;
+  typedef typename El<TY>::Frag Frag;
+  constexpr int QT = 32;
+  typedef Tile<TY, DQ> TQ;
+  typedef Tile<TY, DV> TG;
+  constexpr int QB = MAPS * QT * TQ::ROWB, GB = QT * TG::ROWB, SB = 3 * MAPS * QT * 4, ST = QB + GB + SB;
+  extern __shared__ __align__(16) char smem[];       // 2 x (Q maps, dO, statistics m | lg | delta of each map) | bias table
+  const BwdWork wk(a, MAPS);
+  float* tab = reinterpret_cast<float*>(smem + 2 * ST);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
+  const int bh = blockIdx.x % (a.B * a.Hkv), b = bh / a.Hkv, hk = bh % a.Hkv, blk = blockIdx.x / (a.B * a.Hkv);
+  const int G = a.H / a.Hkv;
+  const int nq = clamp_len(a.q_len, b, a.Lq), nk = clamp_len(a.kv_len, b, a.Lk), st = start_of(a.q_start, b);
+  const int blk0 = blk * 128;
+  if (blk0 >= nk) return;
+  const int key0 = blk0 + wave * 32, key = key0 + li;
+  const bool ok = key < nk;
+  float lam = 0.0f;
+  if constexpr (MAPS == 2) {
+    float e1, e2;
+    lam = diff_lambda<TY>(a, e1, e2);
+  }
+  Frag kf[MAPS][DQ / 16], vf[DV / 16];
+  {
+    const T* kp = (const T*)a.k + b * a.sk[0] + key * a.sk[1] + hk * a.sk[2];
+    const T* vp = (const T*)a.v + b * a.sv[0] + key * a.sv[1] + hk * a.sv[2];
+#pragma unroll
+    for (int p = 0; p < MAPS; ++p)
+#pragma unroll
+      for (int s = 0; s < DQ / 16; ++s) {
+        const int d = 16 * s + 8 * half;
+        kf[p][s] = global_frag<TY>(kp + (MAPS == 2 ? p * a.sk[3] : 0) + d, ok && d < a.D);
+      }
+#pragma unroll
+    for (int s = 0; s < DV / 16; ++s) {
+      const int d = 16 * s + 8 * half;
+      vf[s] = global_frag<TY>(vp + d, ok && d < a.Dv);
+    }
+  }
+  float rs = 1.0f;
+  if constexpr (TY == TY_F16) {
+    float top = 0.0f;
+    for (int i = lane; i < G * wk.nblk; i += 64) top = fmaxf(top, a.ws[wk.top + ((long)b * a.H + hk * G) * wk.nblk + i]);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    rs = pow2_to_one(top);
+  }
+  f32x16 dk[MAPS][DQ / 32], dv[DV / 32];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+#pragma unroll
+    for (int p = 0; p < MAPS; ++p)
+#pragma unroll
+      for (int d = 0; d < DQ / 32; ++d) dk[p][d][r] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DV / 32; ++d) dv[d][r] = 0.0f;
+  }
+  const float c2 = a.scale * LOG2E;
+  // under a causal mask the first query that sees key blk0 stands at its position
+  const int q_first = a.causal ? min(max(blk0 - st, 0), nq) / QT * QT : 0;
+  const int nt = nq > q_first ? (nq - q_first + QT - 1) / QT : 0;
+  const int wave_first = a.causal ? key0 - st : 0;    // first query that sees any of this wave's keys
+
+  Stage<TY, DQ, QT, 256> qs[MAPS];
+  Stage<TY, DV, QT, 256> gs;
+  float sv = 0.0f;                                    // thread tid < 3 MAPS QT: one statistic of the tile
+  auto fetch = [&](int it) {
+    const int h = hk * G + it / nt, r0 = q_first + it % nt * QT;
+    const T* qp = (const T*)a.q + b * a.sq[0] + h * a.sq[2];
+    const T* gp = (const T*)a.dout + b * a.sdo[0] + h * a.sdo[2];
+#pragma unroll
+    for (int p = 0; p < MAPS; ++p) qs[p].load(qp + (MAPS == 2 ? p * a.sq[3] : 0), a.sq[1], r0, nq, a.D, tid);
+    gs.load(gp, a.sdo[1], r0, nq, a.Dv, tid);
+    if (tid < 3 * MAPS * QT) {
+      const int what = tid / QT, p = what / 3, kind = what % 3, row = r0 + tid % QT;
+      const long at = (((long)p * a.B + b) * a.H + h) * a.Lq + row;
+      // a row that is none: weights of exp2(-inf)
+      sv = row >= nq ? (kind == 1 ? INFINITY : 0.0f) : kind == 2 ? a.ws[wk.delta + at] : a.stats[2 * at + kind];
+    }
+  };
+  auto put = [&](int buf) {
+    char* base = smem + buf * ST;
+#pragma unroll
+    for (int p = 0; p < MAPS; ++p) qs[p].store(base + p * QT * TQ::ROWB, tid);
+    gs.store(base + QB, tid);
+    if (tid < 3 * MAPS * QT) reinterpret_cast<float*>(base + QB + GB)[tid] = sv;
+  };
+  const int steps = nt * G;
+  int filled = -1;
+  if (steps > 0) {
+    fetch(0);
+    put(0);
+  }
+  float far_l = 0.0f, far_r = 0.0f;
+  bool fold = true;
+  for (int it = 0; it < steps; ++it) {
+    const int h = hk * G + it / nt, r0 = q_first + it % nt * QT;
+    if (BIAS && filled != h) {
+      // every wave is past its last read of the table: the barrier at the end of the step before
+      fill_bias<TY>(a, tab, h, tid, 256);
+      far_l = bias_log2<TY>(a, -a.reach, h);
+      far_r = bias_log2<TY>(a, a.reach, h);
+      fold = fabsf(far_l) < BIAS_FOLD && fabsf(far_r) < BIAS_FOLD;
+      filled = h;
+    }
+    if (it == 0 || (BIAS && it % nt == 0)) __syncthreads();
+    const char* qt = smem + (it & 1) * ST;
+    const char* gt = qt + QB;
+    const float* stat = reinterpret_cast<const float*>(gt + GB);
+    if (it + 1 < steps) fetch(it + 1);
+    if (key0 < nk && r0 + QT - 1 >= wave_first) {
+      f32x16 x;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < DV / 16; ++k) x = El<TY>::mma(TG::read_rows(gt, li, k, half), vf[k], x);
+      const bool diag = a.causal && r0 < key0 + 31 - st;             // some pair of the tile is masked
+      const int first = key - st - r0 - 4 * half;                    // register rows from here on see this lane's key
+      f32x16 w0;
+      Frag dsf[MAPS][2];
+#pragma unroll
+      for (int p = 0; p < MAPS; ++p) {
+        f32x16 s;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < DQ / 16; ++k) s = El<TY>::mma(TQ::read_rows(qt + p * QT * TQ::ROWB, li, k, half), kf[p][k], s);
+        bool left = false, right = false;
+        if constexpr (BIAS) {
+          left = key0 + 31 - (st + r0) <= -a.reach;
+          right = key0 - (st + r0 + QT - 1) >= a.reach;
+        }
+        const float* tp = tab + a.reach + BIAS_PAD + (key - st - r0 - 4 * half);
+        const float far = left ? far_l : far_r;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const f32x4 m4 = *reinterpret_cast<const f32x4*>(stat + (3 * p) * QT + 8 * c + 4 * half);
+          const f32x4 l4 = *reinterpret_cast<const f32x4*>(stat + (3 * p + 1) * QT + 8 * c + 4 * half);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float e;
+            if (!BIAS) e = fmaf(s[4 * c + r], c2, -m4[r] - l4[r]);
+            else if ((left || right) && fold) e = fmaf(s[4 * c + r], c2, (far - m4[r]) - l4[r]);
+            else e = (fmaf(s[4 * c + r], c2, (left || right) ? far : tp[-(8 * c + r)]) - m4[r]) - l4[r];
+            if (diag) e = 8 * c + r >= first ? e : -INFINITY;
+            s[4 * c + r] = exp2_(e);
+          }
+        }
+        // P (for dV) and dS
+        if (MAPS == 2 && p == 1) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] *= -lam;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) w0[r] = p == 0 ? s[r] : w0[r] + s[r];
+        f32x16 ds;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const f32x4 d4 = *reinterpret_cast<const f32x4*>(stat + (3 * p + 2) * QT + 8 * c + 4 * half);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) ds[4 * c + r] = s[4 * c + r] * (TY == TY_F16 ? fmaf(x[4 * c + r], rs, -d4[r] * rs) : x[4 * c + r] - d4[r]);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          f32x8 t;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) t[r] = ds[8 * k + r];
+          dsf[p][k] = El<TY>::frag(t);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        f32x8 t;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) t[r] = w0[8 * k + r];
+        const Frag pf = El<TY>::frag(t);
+#pragma unroll
+        for (int d = 0; d < DV / 32; ++d) dv[d] = El<TY>::mma(TG::read_cols(gt, 16 * k, d, lane), pf, dv[d]);
+#pragma unroll
+        for (int p = 0; p < MAPS; ++p)
+#pragma unroll
+          for (int d = 0; d < DQ / 32; ++d) dk[p][d] = El<TY>::mma(TQ::read_cols(qt + p * QT * TQ::ROWB, 16 * k, d, lane), dsf[p][k], dk[p][d]);
+      }
+    }
+    if (it + 1 < steps) put((it & 1) ^ 1);
+    __syncthreads();
+  }
+  if (!ok) return;
+  T* ko = (T*)a.dk + b * a.sdk[0] + key * a.sdk[1] + hk * a.sdk[2];
+  T* vo = (T*)a.dv + b * a.sdv[0] + key * a.sdv[1] + hk * a.sdv[2];
+  const float f = a.scale / rs;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+#pragma unroll
+    for (int p = 0; p < MAPS; ++p)
+#pragma unroll
+      for (int d = 0; d < DQ / 32; ++d) {
+        const int col = 32 * d + 8 * c + 4 * half;
+        f32x4 y = {dk[p][d][4 * c] * f, dk[p][d][4 * c + 1] * f, dk[p][d][4 * c + 2] * f, dk[p][d][4 * c + 3] * f};
+        if (col < a.D) El<TY>::store4(ko + (MAPS == 2 ? p * a.sdk[3] : 0) + col, y);
+      }
+#pragma unroll
+    for (int d = 0; d < DV / 32; ++d) {
+      const int col = 32 * d + 8 * c + 4 * half;
+      f32x4 y = {dv[d][4 * c], dv[d][4 * c + 1], dv[d][4 * c + 2], dv[d][4 * c + 3]};
+      if (col < a.Dv) El<TY>::store4(vo + col, y);
+    }
+  }
+}
+
+// One work-group a head: sums by distance over samples and query blocks, then by bucket.
+template <int TY>
+__global__ __launch_bounds__(1024) void rel_dw_kernel(AttnArgs a) {
+  typedef typename El<TY>::T T;
+  const BwdWork wk(a, 1);
+  __shared__ float by[2 * (1024 + BIAS_PAD) + 1];
+  const int h = blockIdx.x, tid = threadIdx.x;
+  for (int i = tid; i < wk.nrel; i += 1024) {
+    float v = 0.0f;
+    for (int b = 0; b < a.B; ++b) {
+      const float* p = a.ws + wk.part + ((long)(b * a.H + h) * wk.nblk) * wk.nrel + i;
+      float t = 0.0f;
+      for (int c = 0; c < wk.nblk; ++c) t += p[(long)c * wk.nrel];
+      v += t;
+    }
+    by[i] = v;
+  }
+  __syncthreads();
+  for (int k = tid; k < a.num_buckets; k += 1024) {
+    float v = 0.0f;
+    for (int i = 0; i < wk.nrel; ++i) {
+      const int rel = min(max(i - a.reach - BIAS_PAD, -a.reach), a.reach);
+      if (a.lut[rel + a.reach] == k) v += by[i];
+    }
+    El<TY>::store((T*)a.dw + (long)k * a.H + h, v);
+  }
+}
+
+// dlambda over all work-groups, then the four vectors
+template <int TY>
+__global__ __launch_bounds__(256) void diff_dw_kernel(AttnArgs a) {
+  typedef typename El<TY>::T T;
+  const BwdWork wk(a, 2);
+  __shared__ float red[4];
+  const int tid = threadIdx.x;
+  const long n = (long)a.B * a.H * wk.nblk;
+  float v = 0.0f;
+  for (long i = tid; i < n; i += 256) v += a.ws[wk.part + i];
+  v = wave_sum(v);
+  if ((tid & 63) == 0) red[tid >> 6] = v;
+  __syncthreads();
+  v = -((red[0] + red[1]) + (red[2] + red[3]));
+  float e1, e2;
+  diff_lambda<TY>(a, e1, e2);
+  const T* w = (const T*)a.w;
+  T* o = (T*)a.dw;
+  for (int d = tid; d < a.D; d += 256) {
+    El<TY>::store(o + d, v * e1 * El<TY>::load(w + a.D + d));
+    El<TY>::store(o + a.D + d, v * e1 * El<TY>::load(w + d));
+    El<TY>::store(o + 2 * a.D + d, -v * e2 * El<TY>::load(w + 3 * a.D + d));
+    El<TY>::store(o + 3 * a.D + d, -v * e2 * El<TY>::load(w + 2 * a.D + d));
+  }
+}
+
+template <int TY, int MAPS, int DQ, int DV, bool BIAS> static int launch_bwd(const AttnArgs* a, hipStream_t stream) {
+  constexpr int SZ = sizeof(typename El<TY>::T);
+  const BwdWork wk(*a, MAPS);
+  const int tab = BIAS ? wk.nrel * 4 : 0;
+  constexpr int KT = TY == TY_F32 ? 32 : 64;
+  int lds = 2 * KT * (MAPS * DQ + DV) * SZ + 9 * tab;
+  if (int e = allow_lds<attn_dq_kernel<TY, MAPS, DQ, DV, BIAS>>(lds)) return e;
+  hipLaunchKernelGGL((attn_dq_kernel<TY, MAPS, DQ, DV, BIAS>), dim3(a->B * a->H * wk.nblk), dim3(256), lds, stream, *a);
+  SGTA_LAUNCH_CHECK();
+  const int nblk = cdiv(a->Lk, 128);
+  lds = 2 * (32 * (MAPS * DQ + DV) * SZ + 3 * MAPS * 32 * 4) + tab;
+  if (int e = allow_lds<attn_dkv_kernel<TY, MAPS, DQ, DV, BIAS>>(lds)) return e;
+  hipLaunchKernelGGL((attn_dkv_kernel<TY, MAPS, DQ, DV, BIAS>), dim3(a->B * a->Hkv * nblk), dim3(256), lds, stream, *a, nblk);
+  SGTA_LAUNCH_CHECK();
+  if (MAPS == 1) hipLaunchKernelGGL((rel_dw_kernel<TY>), dim3(a->H), dim3(1024), 0, stream, *a);
+  else hipLaunchKernelGGL((diff_dw_kernel<TY>), dim3(1), dim3(256), 0, stream, *a);
+  SGTA_LAUNCH_CHECK();
+  return SGTA_OK;
+}
+
+static int bwd_check(const AttnArgs* a, int maps) {
+  if (int e = attn_check(a, maps)) return e;
+  if (!a->dout || !a->dq || !a->dk || !a->dv || !a->dw || !a->stats || !a->ws || (maps == 2 && !a->out2)) return SGTA_EBADARG;
+  if (a->ws_floats < BwdWork(*a, maps).total) return SGTA_EBADARG;
+  const int al = a->dtype == TY_F32 ? 4 : 8;
+  const long* s[] = {a->sdo, a->sdq, a->sdk, a->sdv};
+  const void* p[] = {a->dout, a->dq, a->dk, a->dv};
+  for (int i = 0; i < 4; ++i) {
+    if ((uintptr_t)p[i] % 16) return SGTA_EBADARG;
+    for (int j = 0; j < ((i == 1 || i == 2) && maps == 2 ? 4 : 3); ++j)
+      if (s[i][j] % al) return SGTA_EBADARG;
+  }
+  return SGTA_OK;
+}
+
+extern "C" long sgta_attn_bwd_ws_floats(const sgta_attn_t* a, int maps) {
+  return (maps != 1 && maps != 2) || attn_check(a, maps) ? 0 : BwdWork(*a, maps).total;
+}
+
+template <int TY> static int rel_bwd(const AttnArgs* a, hipStream_t st) {
+  if (a->D <= 32) return launch_bwd<TY, 1, 32, 32, true>(a, st);
+  if (a->D <= 64) return launch_bwd<TY, 1, 64, 64, true>(a, st);
+  return launch_bwd<TY, 1, 128, 128, true>(a, st);
+}
+template <int TY> static int diff_bwd(const AttnArgs* a, hipStream_t st) {
+  return a->D <= 32 && a->Dv <= 64 ? launch_bwd<TY, 2, 32, 64, false>(a, st) : launch_bwd<TY, 2, 64, 128, false>(a, st);
+}
+
+extern "C" int sgta_rel_attn_bwd(const sgta_attn_t* a, sgta_stream_t stream) {
+  if (int e = bwd_check(a, 1)) return e;
+  hipStream_t st = (hipStream_t)stream;
+  return a->dtype == TY_F32 ? rel_bwd<TY_F32>(a, st) : a->dtype == TY_F16 ? rel_bwd<TY_F16>(a, st) : rel_bwd<TY_BF16>(a, st);
+}
+extern "C" int sgta_diff_attn_bwd(const sgta_attn_t* a, sgta_stream_t stream) {
+  if (int e = bwd_check(a, 2)) return e;
+  hipStream_t st = (hipStream_t)stream;
+  return a->dtype == TY_F32 ? diff_bwd<TY_F32>(a, st) : a->dtype == TY_F16 ? diff_bwd<TY_F16>(a, st) : diff_bwd<TY_BF16>(a, st);
+}

@@ -38,16 +38,15 @@ template <> struct El<TY_F32> {
 };
 template <bool F16> struct El16 {
   typedef typename H16<F16>::T T;
+  typedef typename H16<F16>::x4 x4;
   typedef typename H16<F16>::x8 Frag;
   static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) { return H16<F16>::mfma32(a, b, c); }
-  // IEEE half: values beyond 65504 are clamped, as everywhere in the 16-bit data path
-  static __device__ __forceinline__ Frag frag(f32x8 v) { return H16<F16>::cvt8(v); }
+  // to the nearest, without the clamp of the 16-bit feature maps: here what exceeds the half range becomes an infinity, by which
+  // a training loop sees that its loss is scaled too far
+  static __device__ __forceinline__ Frag frag(f32x8 v) { return __builtin_convertvector(v, Frag); }
   static __device__ __forceinline__ float load(const T* p) { return (float)*p; }
-  static __device__ __forceinline__ void store4(T* p, f32x4 v) { *reinterpret_cast<typename H16<F16>::x4*>(p) = H16<F16>::cvt4(v); }
-  static __device__ __forceinline__ void store(T* p, float v) {
-    f32x4 t = {v, 0.0f, 0.0f, 0.0f};
-    *p = H16<F16>::cvt4(t)[0];
-  }
+  static __device__ __forceinline__ void store4(T* p, f32x4 v) { *reinterpret_cast<x4*>(p) = __builtin_convertvector(v, x4); }
+  static __device__ __forceinline__ void store(T* p, float v) { *p = (T)v; }
 };
 template <> struct El<TY_F16> : El16<true> {};
 template <> struct El<TY_BF16> : El16<false> {};
@@ -128,8 +127,7 @@ template <int TY, int COLS> struct Tile {
 template <int TY, int COLS, int ROWS, int NT> struct Stage {
   typedef Tile<TY, COLS> Tl;
   typedef typename El<TY>::T T;
-  static constexpr int N = ROWS * Tl::CH / NT;
-  static_assert(ROWS * Tl::CH % NT == 0, "whole pieces per thread");
+  static constexpr int ALL = ROWS * Tl::CH, N = (ALL + NT - 1) / NT;
   u32x4 r[N];
   __device__ __forceinline__ void load(const T* p, long ld, int row0, int rows, int cols, int tid) {
 #pragma unroll
@@ -137,14 +135,14 @@ template <int TY, int COLS, int ROWS, int NT> struct Stage {
       const int c = tid + i * NT, row = row0 + c / Tl::CH, e = (c % Tl::CH) * Tl::EPC;
       u32x4 z = {0, 0, 0, 0};
       r[i] = z;
-      if (row < rows && e < cols) r[i] = *reinterpret_cast<const u32x4*>(p + (long)row * ld + e);
+      if ((ALL % NT == 0 || c < ALL) && row < rows && e < cols) r[i] = *reinterpret_cast<const u32x4*>(p + (long)row * ld + e);
     }
   }
   __device__ __forceinline__ void store(char* lds, int tid) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int c = tid + i * NT;
-      *reinterpret_cast<u32x4*>(lds + Tl::piece(c / Tl::CH, c % Tl::CH)) = r[i];
+      if (ALL % NT == 0 || c < ALL) *reinterpret_cast<u32x4*>(lds + Tl::piece(c / Tl::CH, c % Tl::CH)) = r[i];
     }
   }
 };
@@ -196,13 +194,14 @@ template <int TY> __device__ __forceinline__ void fill_bias(const AttnArgs& a, f
 // beyond this a bias absorbs the scores it is added to: such tiles add it to each score instead of folding it into the exponent
 #define BIAS_FOLD 1e30f
 
-// lets a kernel use up to 160 KB of LDS on the current device (once a device), refuses more
+// lets a kernel use up to 158 KB of dynamic LDS on the current device (once a device; 2 KB of the 160 are left for static arrays),
+// refuses more
 template <auto KERNEL> static int allow_lds(int bytes) {
   static bool done[SGTA_MAX_DEVICES];
-  if (bytes > 160 * 1024) return SGTA_EBADARG;
+  if (bytes > 158 * 1024) return SGTA_EBADARG;
   const int slot = sgta_device_slot();
   if (!done[slot]) {
-    const hipError_t e = hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    const hipError_t e = hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, 158 * 1024);
     if (e != hipSuccess) return (int)e;
     done[slot] = true;
   }

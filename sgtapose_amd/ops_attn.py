@@ -236,3 +236,52 @@ def diff_attention(q, k, v, lam, out=None, *, lam_init=0.8, causal=False, scale=
     a.lam_init = lam_init
     with torch.cuda.device(q.device):
         return _forward("sgta_diff_attn_fwd", 2, a, q, out, q_len, save)
+
+
+def _backward(name, maps, a, like, dout, w, out, saved, grads, q_len, kv_len):
+    mp = (2,) if maps == 2 else ()
+    stats, out2 = saved
+    shape = (a.B, a.Lq, a.H, a.Dv)
+    _layout("dout", dout, shape, like)
+    _layout("out", out, shape, like)
+    if tuple(stats.shape) != (maps, a.B, a.H, a.Lq, 2) or stats.device != like.device or (maps == 2 and tuple(out2.shape) != shape):
+        _fail("saved does not come from a forward call of this shape")
+    dq, dk, dv, dw = grads
+    dq = _output("dq", dq, (a.B, a.Lq, a.H, *mp, a.D), like, q_len is not None)
+    dk = _output("dk", dk, (a.B, a.Lk, a.Hkv, *mp, a.D), like, kv_len is not None)
+    dv = _output("dv", dv, (a.B, a.Lk, a.Hkv, a.Dv), like, kv_len is not None)
+    if dw is None:
+        dw = torch.empty_like(w)
+    elif dw.shape != w.shape or dw.dtype != w.dtype or dw.device != w.device or not dw.is_contiguous():
+        _fail("the learned weights' gradient is %s %s, expected %s %s, contiguous", dw.dtype, tuple(dw.shape), w.dtype, tuple(w.shape))
+    g, o, q_, k_, v_ = (_dense(t) for t in (dout, out, dq, dk, dv))
+    a.dout, a.sdo, a.out, a.so = g.data_ptr(), _strides(g, 1), o.data_ptr(), _strides(o, 1)
+    a.dq, a.sdq, a.dk, a.sdk, a.dv, a.sdv = q_.data_ptr(), _strides(q_, maps), k_.data_ptr(), _strides(k_, maps), v_.data_ptr(), _strides(v_, 1)
+    a.dw, a.stats, a.out2 = dw.data_ptr(), stats.data_ptr(), _ptr(out2)
+    ws = _work(_lib.load().sgta_attn_bwd_ws_floats(ctypes.byref(a), maps), like.device)
+    a.ws, a.ws_floats = ws.data_ptr(), ws.numel()
+    _enqueue(name, a, like.device, _meta(name, a, maps, (5 * maps, 3)))
+    return dq, dk, dv, dw
+
+
+def rel_attention_bwd(dout, q, k, v, table, out, saved, dq=None, dk=None, dv=None, dtable=None, *, max_distance=128, bidirectional=True,
+                      causal=False, scale=None, q_len=None, kv_len=None, q_start=None):
+    """Gradients (dq, dk, dv, dtable) of ``rel_attention`` for the gradient ``dout`` of its ``out``; the other arguments as in the
+    forward call, ``saved`` from its ``save=True``.  Shared heads' gradients are summed; rows behind q_len / kv_len are left as they
+    are (zeros where allocated here).  The same inputs give the same bits."""
+    reach = _check_table(table, q.shape[2], max_distance, bidirectional)
+    a = _operands(1, q, k, v, table, causal, scale, q_len, kv_len, q_start)
+    with torch.cuda.device(q.device):
+        lut = _lut(table.shape[0], int(max_distance), bool(bidirectional), q.device)
+        a.lut, a.reach, a.num_buckets = lut.data_ptr(), reach, table.shape[0]
+        return _backward("sgta_rel_attn_bwd", 1, a, q, dout, table, out, saved, (dq, dk, dv, dtable), q_len, kv_len)
+
+
+def diff_attention_bwd(dout, q, k, v, lam, out, saved, dq=None, dk=None, dv=None, dlam=None, *, lam_init=0.8, causal=False, scale=None,
+                       q_len=None, kv_len=None, q_start=None):
+    """Gradients (dq, dk, dv, dlam) of ``diff_attention``, as ``rel_attention_bwd``; dlam [4, D]."""
+    _check_lam(lam, q.shape[-1])
+    a = _operands(2, q, k, v, lam, causal, scale, q_len, kv_len, q_start)
+    a.lam_init = lam_init
+    with torch.cuda.device(q.device):
+        return _backward("sgta_diff_attn_bwd", 2, a, q, dout, lam, out, saved, (dq, dk, dv, dlam), q_len, kv_len)

@@ -6,6 +6,10 @@ Tolerances are bounds, element by element, from the arithmetic of the kernels (u
   weights   rounded to the element type before the product with v: u of each (IEEE half: 2^-25 at least, where it is subnormal)
   sums      Lk terms in f32: e Lk of the sum of magnitudes
   output    rounded once more: u |o|
+Gradients, with a = 4 es + e Lk for the relative error of a weight from the saved statistics:
+  X = dO V^T   e (Dv + 2) |dO||V|^T;   delta: |dO| times the output's bound, and e (Dv + 2) |dO||O|
+  dS           a |dS| + P (X's + delta's); rounded to the element type: u |dS| (IEEE half: scaled to |dO| next to one, so 2^-24 of it at least)
+  dQ, dK, dV   the sums of those errors times the other operand's magnitude, e per term of the sum, u of the result
 """
 import math
 
@@ -118,12 +122,77 @@ class Case:
         return r
 
 
+def gradients(c):
+    """-> {name: (gradient, bound)} in float64 for c.dout (after c.reference())."""
+    r = c.reference()
+    z = c.parts
+    B, Lq, Lk, H, Hkv, D, Dv = c.dims
+    G, u, P, v, do, lam = H // Hkv, z["u"], z["P"], z["v"], z["do"], z["lam"]
+    X, Xe = do @ v.transpose(-1, -2), E * (Dv + 2) * (do.abs() @ v.abs().transpose(-1, -2))
+    top = do.abs().amax() * 2
+    tiny = 2.0 ** -24 * top if c.dtype == torch.float16 else 0.0
+    sgn = (1.0, -lam)
+    o = [P[p] @ v for p in range(c.maps)]
+    out = sum(sgn[p] * o[p] for p in range(c.maps))
+    a = [4 * e + z["sums"] + 16 * E for e in z["es"]]
+    dsum = lambda t: (do.abs() * t).sum(-1, keepdim=True)                                         # noqa: E731
+    d_err = dsum(z["o_mid"] + u * out.abs()) + E * (Dv + 2) * dsum(out.abs())
+    res, dS, Se = {}, [], []
+    d2 = d2_err = None
+    if c.maps == 2:
+        d2 = (do * o[1]).sum(-1, keepdim=True)
+        d2_err = dsum((u + a[1]) * (P[1] @ v.abs()) + z["tiny"] * (z["seen"].double() @ v.abs()) + u * o[1].abs()) + E * (Dv + 2) * dsum(o[1].abs())
+        d_err = d_err + abs(lam) * d2_err
+    for p in range(c.maps):
+        d = (do * o[p]).sum(-1, keepdim=True)
+        t = sgn[p] * P[p] * (X - d)
+        dS.append(t)
+        Se.append(a[p] * t.abs() + abs(sgn[p]) * P[p] * (Xe + (d_err if p == 0 else d2_err)) + (8 * E * t.abs() if c.maps == 2 else 0.0))
+    shared = lambda t: t.reshape(B, Hkv, G, *t.shape[2:]).sum(2)                                  # noqa: E731
+    back = lambda t: t.transpose(1, 2)                                                            # noqa: E731
+
+    def pack(name, parts):
+        val, err = (torch.stack([x[i] for x in parts], 3) if c.maps == 2 and name != "dv" else parts[0][i] for i in (0, 1))
+        # a half below 2^-14 has steps of 2^-24 whatever its size, so its rounding is off by up to 2^-25 rather than u of it
+        res[name] = (val, err * 1.01 + u * val.abs() + 2 * E * val.abs() + FLUSH[c.dtype] + 1e-30)
+    dq, dk = [], []
+    for p in range(c.maps):
+        k, q, m = z["k"][p], z["q"][p], dS[p].abs()
+        e = Se[p] + (u + Lk * E) * m + tiny
+        dq.append((back(z["c"] * (dS[p] @ k)), back(z["c"] * (e @ k.abs()))))
+        e = Se[p] + (u + Lq * G * E) * m + tiny
+        dk.append((back(shared(z["c"] * (dS[p].transpose(-1, -2) @ q))), back(shared(z["c"] * (e.transpose(-1, -2) @ q.abs())))))
+    w = sum(sgn[p] * P[p] for p in range(c.maps))
+    we = sum(abs(sgn[p]) * a[p] * P[p] for p in range(c.maps)) + (u + Lq * G * E) * sum(abs(sgn[p]) * P[p] for p in range(c.maps)) + z["tiny"]
+    if c.maps == 2:
+        we = we + 1e-5 * P[1]
+    pack("dq", dq)
+    pack("dk", dk)
+    pack("dv", [(back(shared(w.transpose(-1, -2) @ do)), back(shared(we.transpose(-1, -2) @ do.abs())))])
+    if c.maps == 1:
+        hit = torch.nn.functional.one_hot(z["of"], c.buckets).double()                            # [B, Lq, Lk, buckets]
+        tot = lambda t: torch.einsum("bhij,bijn->nh", t, hit)                                     # noqa: E731
+        val, err = tot(dS[0]), tot(Se[0] + (Lk + 200) * E * dS[0].abs())
+    else:
+        wt = c.w.double()
+        e1, e2 = torch.exp((wt[0] * wt[1]).sum()), torch.exp((wt[2] * wt[3]).sum())
+        dl, de = -d2.sum(), (d2_err + 300 * E * d2.abs()).sum()
+        val = torch.stack([dl * e1 * wt[1], dl * e1 * wt[0], -dl * e2 * wt[3], -dl * e2 * wt[2]])
+        err = (de + 1e-5 * dl.abs()) * torch.stack([e1 * wt[1].abs(), e1 * wt[0].abs(), e2 * wt[3].abs(), e2 * wt[2].abs()])
+    res["dw"] = (val, err * 1.01 + u * val.abs() + 4 * E * val.abs() + FLUSH[c.dtype] + 1e-30)
+    return r, res
+
+
 def within(name, got, want, tol, rows=None):
     d = (got.double().cpu() - want).abs()
+    tol_all = tol
     if rows is not None:
         keep = torch.arange(got.shape[1])[None] < rows[:, None]
         d, tol = d[keep], tol.expand(want.shape)[keep]
     bad = ~(d <= tol)
+    # what exceeds the type's range becomes an infinity of its sign: right where the value, give or take its bound, does
+    beyond = got.double().cpu().isinf() & (want * got.double().cpu().sign() + tol_all >= torch.finfo(got.dtype).max)
+    bad &= ~(beyond if rows is None else beyond[keep])
     assert not bad.any(), "%s: %d of %d beyond the bound, worst %.3g against %.3g" % (
         name, int(bad.sum()), bad.numel(), float(d[bad].max()), float(tol.expand(d.shape)[bad].min()))
 
@@ -139,6 +208,28 @@ def check_forward(c):
     torch.cuda.synchronize()
     within("out", got, r["out"], r["out_tol"], r["nq"])
     return got
+
+
+def both_ways(c, dev="cuda", **grads):
+    t = [x.to(dev) for x in (c.q, c.k, c.v, c.w)]
+    kw = c.kwargs(dev)
+    fwd, bwd = ((ops_attn.rel_attention, ops_attn.rel_attention_bwd) if c.maps == 1 else (ops_attn.diff_attention, ops_attn.diff_attention_bwd))
+    out, saved = fwd(*t, **kw, save=True)
+    return out, bwd(c.dout.to(dev), *t, out, saved, **kw, **grads)
+
+
+def check_both(c):
+    r, want = gradients(c)
+    out, got = both_ways(c)
+    torch.cuda.synchronize()
+    within("out", out, r["out"], r["out_tol"], r["nq"])
+    rows = dict(dq=r["nq"], dk=r["nk"], dv=r["nk"])
+    for name, g in zip(("dq", "dk", "dv", "dw"), got):
+        within(name, g, *want[name], rows.get(name))
+        if name in rows:
+            behind = torch.arange(g.shape[1])[None] >= rows[name][:, None]
+            assert bool((g.cpu()[behind] == 0).all()), name
+    return out, got
 
 
 # ---- host ---------------------------------------------------------------------------------------
@@ -353,3 +444,149 @@ def test_streams_and_graphs():
                 g.replay()
                 torch.cuda.synchronize()
                 assert torch.equal(out, want)
+
+
+# ---- gradients ------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dtype", ALL, ids=NAMES.get)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_rel_gradients(dtype, causal, shape):
+    B, Lq, Lk, H, Hkv = shape
+    for D in (16, 64, 128):
+        check_both(Case(1, dtype, B, Lq, Lk, H, Hkv, D, causal=causal, seed=D, q_start=[max(0, Lk - Lq)] * B if causal else None))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ALL, ids=NAMES.get)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_diff_gradients(dtype, causal, shape):
+    B, Lq, Lk, H, Hkv = shape
+    for D, Dv in ((16, 32), (64, 128), (40, 24)):
+        check_both(Case(2, dtype, B, Lq, Lk, H, Hkv, D, Dv, causal=causal, seed=D, q_start=[max(0, Lk - Lq)] * B if causal else None))
+
+
+@gpu
+@pytest.mark.parametrize("maps", [1, 2])
+@pytest.mark.parametrize("dtype", ALL, ids=NAMES.get)
+def test_gradients_lengths_and_starts(maps, dtype):
+    for causal in (False, True):
+        for Lq in (3, 150):
+            c = Case(maps, dtype, 6, Lq, 200, 4, 2, 32, causal=causal, kv_len=[0, 1, 200, 77, 128, 500], seed=Lq,
+                     q_len=[Lq, Lq, 0, max(1, Lq // 2), Lq, Lq + 9], q_start=[0, 0, 3, 76, -5, 2 ** 30 + 5])
+            want_out, want = both_ways(c)
+            for b in range(6):                                       # what lies behind the lengths takes no part
+                for t in (c.k, c.v):
+                    t[b, min(200, c.lens["kv_len"][b]):] = math.nan
+                for t in (c.q, c.dout):
+                    t[b, min(Lq, c.lens["q_len"][b]):] = math.nan
+            out, got = check_both(c)
+            assert torch.equal(out, want_out) and all(torch.equal(x, y) for x, y in zip(got, want))
+            # gradients into the caller's tensors: rows behind the lengths stay as they are
+            mine = [torch.full_like(x, 3.0) for x in got]
+            names = ("dq", "dk", "dv", "dtable" if maps == 1 else "dlam")
+            _, into = both_ways(c, **dict(zip(names, mine)))
+            for name, x, y, n in zip(names, into, got, (c.parts["nq"], c.parts["nk"], c.parts["nk"], None)):
+                if n is None:
+                    assert torch.equal(x, y)
+                    continue
+                keep = (torch.arange(x.shape[1])[None] < n[:, None]).cuda()
+                assert torch.equal(x[keep], y[keep]) and bool((x[~keep] == 3.0).all()), name
+
+
+@gpu
+@pytest.mark.parametrize("maps", [1, 2])
+@pytest.mark.parametrize("size", [1e-5, 1e4])
+def test_half_gradients_of_any_magnitude(maps, size):
+    """dO far from one: IEEE half keeps its relative accuracy (dV's operand is dO itself)."""
+    check_both(Case(maps, torch.float16, 1, 200, 300, 2, 1, 32, seed=3, dout_scale=size))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ALL, ids=NAMES.get)
+def test_rel_gradients_table_infinities_and_lowest_values(dtype):
+    for causal in (False, True):
+        for value in (-math.inf, torch.finfo(dtype).min):
+            c = Case(1, dtype, 1, 200, 300, 2, 2, 32, causal=causal, q_start=[100] if causal else None)
+            c.w[::2] = value
+            check_both(c)
+        c.w[:] = torch.finfo(dtype).min                              # equal weights everywhere
+        check_both(c)
+
+
+@gpu
+@pytest.mark.parametrize("buckets,far", [(2, 2), (16, 64), (64, 1024), (128, 100)])
+def test_rel_gradients_bucket_tables(buckets, far):
+    for causal in (False, True):
+        if not causal and buckets == 2:
+            continue
+        check_both(Case(1, torch.bfloat16, 2, 140, 260, 2, 1, 32, causal=causal, buckets=buckets, far=far, q_start=[120, 7] if causal else None))
+
+
+@gpu
+@pytest.mark.parametrize("maps", [1, 2])
+def test_gradients_against_differences(maps):
+    """Central differences of the 64-bit formula along random directions."""
+    c = Case(maps, torch.float32, 2, 9, 40, 2, 1, 16, causal=True, q_start=[31, 20], kv_len=[40, 25], seed=4)
+    r, want = gradients(c)
+    _, got = both_ways(c)
+    g = torch.Generator().manual_seed(1)
+    h = 1e-4
+    for name, at in (("dq", "q"), ("dk", "k"), ("dv", "v"), ("dw", "w")):
+        base = getattr(c, at)
+        d = torch.randn(base.shape, generator=g, dtype=torch.float64)
+        side = []
+        for sign in (1, -1):
+            setattr(c, at, base.double() + sign * h * d)
+            side.append((c.reference()["out"] * c.dout.double()).sum())
+        setattr(c, at, base)
+        slope = float((side[0] - side[1]) / (2 * h))
+        mine = got[("dq", "dk", "dv", "dw").index(name)].double().cpu()
+        rest = float((want[name][1] * d.abs()).sum()) + 1e-5 * float((mine * d).abs().sum())       # the bound; h^2 of the third derivative
+        assert abs(slope - float((mine * d).sum())) <= rest, (name, slope, float((mine * d).sum()), rest)
+
+
+@gpu
+@pytest.mark.parametrize("maps", [1, 2])
+def test_gradients_repeat_and_replay(maps):
+    """The same inputs give the same bits, eager, on another stream, and from a graph replayed between eager work."""
+    c = Case(maps, torch.bfloat16, 2, 300, 300, 4, 2, 64, causal=True, seed=8)
+    want_out, want = both_ways(c)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        again_out, again = both_ways(c)
+    s.synchronize()
+    assert torch.equal(again_out, want_out) and all(torch.equal(x, y) for x, y in zip(again, want))
+    t = [x.cuda() for x in (c.q, c.k, c.v, c.w)]
+    do, kw = c.dout.cuda(), c.kwargs("cuda")
+    fwd, bwd = ((ops_attn.rel_attention, ops_attn.rel_attention_bwd) if maps == 1 else (ops_attn.diff_attention, ops_attn.diff_attention_bwd))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, saved = fwd(*t, **kw, save=True)
+        grads = bwd(do, *t, out, saved, **kw)
+    for n in range(3):
+        t[0].copy_(c.q * (1 + n))
+        o, sv = fwd(*t, **kw, save=True)
+        fresh = bwd(do, *t, o, sv, **kw)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, out) and all(torch.equal(x, y) for x, y in zip(fresh, grads))
+
+
+def test_backward_refuses():
+    z = _cpu()
+    out = torch.zeros(2, 5, 4, 16, dtype=torch.bfloat16)
+    with pytest.raises(SgtaHipError, match="GPU"):
+        ops_attn.rel_attention_bwd(out, *z, out, (torch.zeros(1, 2, 4, 5, 2), None))
+    import ctypes
+    from sgtapose_amd import _lib
+    lib = _lib.load()
+    ok = dict(q=64, k=64, v=64, w=64, out=64, lut=64, B=1, Lq=4, Lk=4, H=2, Hkv=2, D=16, Dv=16, dtype=2, reach=8, num_buckets=8, scale=0.25,
+              dout=64, dq=64, dk=64, dv=64, dw=64, stats=64, ws=64, ws_floats=1 << 20)
+    for change in (dict(dout=None), dict(dq=None), dict(dw=None), dict(stats=None), dict(ws=None), dict(ws_floats=3), dict(dk=65), dict(D=12),
+                   dict(sdv=(ctypes.c_long * 4)(16, 4, 16, 0))):
+        a = _lib.AttnArgs(**{**ok, **change})
+        assert lib.sgta_rel_attn_bwd(ctypes.byref(a), None) < 0, change
+    assert lib.sgta_diff_attn_bwd(ctypes.byref(_lib.AttnArgs(**ok)), None) < 0      # no second map's product
