@@ -502,7 +502,9 @@ int sgta_dcnv2_x3(const float* x, long x_bs, const float* om, long om_bs, const 
  * Strides in elements {batch, position, head, map}; the last dimension is contiguous; strides whole 16 bytes, pointers 16-byte
  * aligned.  D, Dv multiples of 8; one map: D = Dv <= 128; two maps: D <= 64, Dv <= 128.  H % Hkv == 0.  q_len / kv_len /
  * q_start int32 [B] or NULL (Lq, Lk, 0).  w: table [num_buckets, H] or the four vectors [4, D], contiguous.
- * lut: int32 [2 reach + 1], bucket of each distance; from ``reach`` on (<= 1024) it stays the same.
+ * lut: int32 [2 reach + 1], bucket of each distance; from ``reach`` on (<= 1024) it stays the same.  Behind it, for the backward
+ * pass, first[num_buckets] and count[num_buckets]: each bucket's run of entries (one run each; a count of 0: none).
+ * Positions of q, k, v and dout lie at most 16 MB apart (strides [1]).
  * stats: f32 [maps][B][H][Lq][2] (reference and log2 of the sum, for the backward pass) or NULL.
  * out2: [B, Lq, H, Dv] contiguous, the second map's product with v (for the backward pass) or NULL.
  * ws: f32 workspace of sgta_attn_fwd_ws_floats() floats (0: not used), written before it is read; calls that may

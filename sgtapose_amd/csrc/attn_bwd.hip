@@ -25,53 +25,70 @@ __device__ __forceinline__ float pow2_to_one(float top) {          // 2^-exponen
 
 // the workspace, in floats
 struct BwdWork {
-  long delta, part, top;       // [maps][B][H][Lq]; per (b, h, query block): sums by distance, or of d2; largest |dO|
+  long delta, part, top;       // [maps][B][H][Lq]; per (b, h, query block): sums by bucket, or of d2; largest |dO|
   long total;
-  int nblk, nrel;
+  int nblk, nsum, nrel;        // query blocks; floats of a part; distances a work-group tells apart
   __host__ __device__ BwdWork(const AttnArgs& a, int maps) {
     nblk = (a.Lq + 127) / 128;
-    nrel = maps == 1 ? 2 * (a.reach + BIAS_PAD) + 1 : 1;
+    nrel = 2 * (a.reach + BIAS_PAD) + 1;
+    nsum = maps == 1 ? a.num_buckets : 1;
     const long blocks = (long)a.B * a.H * nblk;
     delta = 0;
     part = (long)maps * a.B * a.H * a.Lq;
-    top = part + blocks * nrel;
+    top = part + blocks * nsum;
     total = top + blocks;
   }
 };
 
 template <int TY, int MAPS, int DQ, int DV, bool BIAS>
-__global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2) void attn_dq_kernel(AttnArgs a) {
   typedef typename El<TY>::T T;
   typedef typename El<TY>::Frag Frag;
   constexpr int KT = TY == TY_F32 ? 32 : 64;
   typedef Tile<TY, DQ> TK;
   typedef Tile<TY, DV> TV;
-  constexpr int KB = MAPS * KT * TK::ROWB, VB = KT * TV::ROWB;
+  constexpr int MB = KT * TK::ROWB, KB = MAPS * MB, VB = KT * TV::ROWB;
   extern __shared__ __align__(16) char smem[];       // 2 x (K maps, V) | bias table | 4 waves x 2 lane halves of sums by distance
   const BwdWork wk(a, MAPS);
   float* tab = reinterpret_cast<float*>(smem + 2 * (KB + VB));
   float* hist = tab + wk.nrel;
   __shared__ float red[4];
-  const int nblk = wk.nblk, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
+  const int nblk = wk.nblk, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, half = lane >> 5;
   const int bh = blockIdx.x % (a.B * a.H), b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
   const int blk = a.causal ? nblk - 1 - blockIdx.x / (a.B * a.H) : blockIdx.x / (a.B * a.H);
   const int nq = clamp_len(a.q_len, b, a.Lq), nk = clamp_len(a.kv_len, b, a.Lk), st = start_of(a.q_start, b);
   const int blk0 = blk * 128;
-  float* part = a.ws + wk.part + ((long)bh * nblk + blk) * wk.nrel;
+  float* part = a.ws + wk.part + ((long)bh * nblk + blk) * wk.nsum;
   float* topw = a.ws + wk.top + (long)bh * nblk + blk;
   if (blk0 >= nq) {
-    for (int i = tid; i < wk.nrel; i += 256) part[i] = 0.0f;
+    for (int i = tid; i < wk.nsum; i += 256) part[i] = 0.0f;
     if (tid == 0) *topw = 0.0f;
     return;
   }
   const int row0 = blk0 + wave * 32, row = row0 + li;
   const bool ok = row < nq;
+  const int last_row = min(blk0 + 127, nq - 1);
+  const int seen = a.causal ? min(nk, max(st + last_row + 1, 0)) : nk;
+  const int nt = (seen + KT - 1) / KT;
+  const T* kp = (const T*)a.k + b * a.sk[0] + hk * a.sk[2];
+  const T* vp = (const T*)a.v + b * a.sv[0] + hk * a.sv[2];
+  Dma<TY, DQ, KT, 256> kd;
+  Dma<TY, DV, KT, 256> vd;
+  kd.init(a.sk[1], a.D, tid);
+  vd.init(a.sv[1], a.Dv, tid);
+  auto fetch = [&](int j0, int buf) {
+    char* base = smem + buf * (KB + VB);
+#pragma unroll
+    for (int p = 0; p < MAPS; ++p) kd.issue(kp + (MAPS == 2 ? p * a.sk[3] : 0) + j0 * a.sk[1], seen - j0, base + p * MB, wave);
+    vd.issue(vp + j0 * a.sv[1], seen - j0, base + KB, wave);
+  };
+  if (nt > 0) fetch(0, 0);
+
   float lam = 0.0f;
   if constexpr (MAPS == 2) {
     float e1, e2;
     lam = diff_lambda<TY>(a, e1, e2);
   }
-
   // the row's operands, delta and largest |dO|
   Frag q[MAPS][DQ / 16], g[DV / 16];
   float m[MAPS], lg[MAPS], dl[MAPS], top = 0.0f;
@@ -129,8 +146,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     if (tid == 0) *topw = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     if constexpr (MAPS == 2) {
       __syncthreads();
-      float t2 = half == 0 && ok ? dl[1] : 0.0f;
-      t2 = wave_sum(t2);
+      const float t2 = wave_sum(half == 0 && ok ? dl[1] : 0.0f);
       if (lane == 0) red[wave] = t2;
       __syncthreads();
       if (tid == 0) part[0] = (red[0] + red[1]) + (red[2] + red[3]);
@@ -140,8 +156,9 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
   const float irs = 1.0f / rs;
 
   const int pos = st + row, pmin = st + row0, pmax = st + row0 + 31;
-  const int limit = ok ? min(nk - 1, a.causal ? pos : nk - 1) : -1;
-  float far_l = 0.0f, far_r = 0.0f, sum_l = 0.0f, sum_r = 0.0f;
+  const int limit = min(nk - 1, a.causal ? pos : nk - 1), low = min(nk - 1, a.causal ? pmin : nk - 1);
+  // by row: sums of dS over all keys; of dS and P over the keys left and right of ``reach``
+  float far_l = 0.0f, far_r = 0.0f, sum_l = 0.0f, sum_r = 0.0f, sum_n = 0.0f, p_l = 0.0f, p_r = 0.0f;
   bool fold = true;
   const float* tb = tab;
   float* mine = hist;
@@ -155,118 +172,94 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     mine = hist + (2 * wave + half) * wk.nrel + a.reach + BIAS_PAD;
   }
   const float c2 = a.scale * LOG2E;
-  const int last_row = min(blk0 + 127, nq - 1);
-  const int seen = a.causal ? min(nk, max(st + last_row + 1, 0)) : nk;
-  const int nt = (seen + KT - 1) / KT;
-  const int wave_last = a.causal ? min(seen - 1, st + min(row0 + 31, nq - 1)) : seen - 1;
-  const bool active = row0 < nq;
+  const int wave_last = row0 >= nq ? -1 : a.causal ? min(seen - 1, st + min(row0 + 31, nq - 1)) : seen - 1;
 
   f32x16 dq[MAPS][DQ / 32];
 #pragma unroll
   for (int p = 0; p < MAPS; ++p)
 #pragma unroll
-    for (int d = 0; d < DQ / 32; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) dq[p][d][r] = 0.0f;
+    for (int d = 0; d < DQ / 32; ++d) dq[p][d] = zero16();
 
-  const T* kp = (const T*)a.k + b * a.sk[0] + hk * a.sk[2];
-  const T* vp = (const T*)a.v + b * a.sv[0] + hk * a.sv[2];
-  Stage<TY, DQ, KT, 256> ks[MAPS];
-  Stage<TY, DV, KT, 256> vs;
-  auto fetch = [&](int j0) {
-#pragma unroll
-    for (int p = 0; p < MAPS; ++p) ks[p].load(kp + (MAPS == 2 ? p * a.sk[3] : 0), a.sk[1], j0, seen, a.D, tid);
-    vs.load(vp, a.sv[1], j0, seen, a.Dv, tid);
-  };
-  auto put = [&](int buf) {
-    char* base = smem + buf * (KB + VB);
-#pragma unroll
-    for (int p = 0; p < MAPS; ++p) ks[p].store(base + p * KT * TK::ROWB, tid);
-    vs.store(base + KB, tid);
-  };
-  if (nt > 0) {
-    fetch(0);
-    put(0);
-  }
+  dma_wait<0>();
   __syncthreads();
   for (int t = 0; t < nt; ++t) {
     const char* kt = smem + (t & 1) * (KB + VB);
     const char* vt = kt + KB;
-    if (t + 1 < nt) fetch((t + 1) * KT);
+    if (t + 1 < nt) fetch((t + 1) * KT, (t & 1) ^ 1);
 #pragma unroll
     for (int u = 0; u < KT / 32; ++u) {
       const int j0 = t * KT + 32 * u;
-      if (!active || j0 > wave_last) continue;
-      f32x16 x;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = 0.0f;
+      if (j0 > wave_last) continue;
+      const bool masked = low < j0 + 31;
+      const bool left = BIAS && j0 + 31 - pmin <= -a.reach, right = BIAS && j0 - pmax >= a.reach;
+      const bool plain = !masked && (!BIAS || (fold && (left || right)));
+      f32x16 x = zero16();
 #pragma unroll
       for (int k = 0; k < DV / 16; ++k) x = El<TY>::mma(TV::read_rows(vt, 32 * u + li, k, half), g[k], x);
-      const bool masked = __any(limit < j0 + 31);
-      const int last = limit - j0 - 4 * half;
+      Frag df[MAPS][2];
 #pragma unroll
       for (int p = 0; p < MAPS; ++p) {
-        f32x16 s;
+        f32x16 s = zero16();
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+        for (int k = 0; k < DQ / 16; ++k) s = El<TY>::mma(TK::read_rows(kt + p * MB, 32 * u + li, k, half), q[p][k], s);
+        if (plain) {
+          const float add = ((BIAS ? (left ? far_l : far_r) : 0.0f) - m[p]) - lg[p];
 #pragma unroll
-        for (int k = 0; k < DQ / 16; ++k) s = El<TY>::mma(TK::read_rows(kt + p * KT * TK::ROWB, 32 * u + li, k, half), q[p][k], s);
-        float cc = c2, add = -m[p] - lg[p];
-        bool left = false, right = false;
-        if constexpr (BIAS) {
-          left = j0 + 31 - pmin <= -a.reach;
-          right = j0 - pmax >= a.reach;
-          if ((left || right) && fold) {
-            add = ((left ? far_l : far_r) - m[p]) - lg[p];
-          } else {
-            const float* tp = tb + (j0 + 4 * half - pos);
-            cc = 1.0f;
-            add = -lg[p];
+          for (int r = 0; r < 16; ++r) s[r] = exp2_(fmaf(s[r], c2, add));
+        } else {
+          const int last = masked ? limit - j0 - 4 * half : 32;
+          const float far = left ? far_l : far_r;
+          const bool near = BIAS && !left && !right;
+          const float* tp = tb + (j0 + 4 * half - pos);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const float bias = left ? far_l : right ? far_r : tp[8 * (r >> 2) + (r & 3)];
-              s[r] = fmaf(s[r], c2, bias) - m[p];
-            }
+          for (int r = 0; r < 16; ++r) {
+            const int c = 8 * (r >> 2) + (r & 3);
+            const float e = (fmaf(s[r], c2, !BIAS ? 0.0f : near ? tp[c] : far) - m[p]) - lg[p];
+            s[r] = c <= last ? exp2_(e) : 0.0f;
           }
-        }
-        if (masked) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = 8 * (r >> 2) + (r & 3) <= last ? s[r] : -INFINITY;
-        }
-        const float nd = -dl[p] * rs, sg = (MAPS == 2 && p == 1) ? -lam : 1.0f;
-        float tot[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          f32x8 ds;
-#pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            float w = exp2_(fmaf(s[8 * k + r], cc, add));
-            if (MAPS == 2 && p == 1) w *= sg;
-            ds[r] = w * fmaf(x[8 * k + r], rs, nd);
-            if (BIAS) {
-              tot[r & 3] += ds[r];
-              s[8 * k + r] = ds[r];
-            }
-          }
-          const Frag f = El<TY>::frag(ds);
-#pragma unroll
-          for (int d = 0; d < DQ / 32; ++d)
-            dq[p][d] = El<TY>::mma(TK::read_cols(kt + p * KT * TK::ROWB, 32 * u + 16 * k, d, lane), f, dq[p][d]);
         }
         if constexpr (BIAS) {
           if (left || right) {
-            const float all = ((tot[0] + tot[1]) + (tot[2] + tot[3])) * irs;
-            if (left) sum_l += all; else sum_r += all;
-          } else {
+            const float w = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7])) + (((s[8] + s[9]) + (s[10] + s[11])) + ((s[12] + s[13]) + (s[14] + s[15])));
+            if (left) p_l += w; else p_r += w;
+          }
+        }
+        const float sg = (MAPS == 2 && p == 1) ? -lam : 1.0f;
+        float tot[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float d = s[r] * (TY == TY_F16 ? fmaf(x[r], rs, -dl[p] * rs) : x[r] - dl[p]);
+          s[r] = (MAPS == 2 && p == 1) ? d * sg : d;
+          if (BIAS) tot[r & 1] += s[r];
+        }
+        if constexpr (BIAS) {
+          const float all = (tot[0] + tot[1]) * irs;
+          if (left) sum_l += all;
+          else if (right) sum_r += all;
+          else {
+            sum_n += all;
             // one distance a lane and instruction, the lane halves apart: no two lanes add to one place
             float* hp = mine + (j0 + 4 * half - pos);
 #pragma unroll
             for (int r = 0; r < 16; ++r) __hip_atomic_fetch_add(hp + 8 * (r >> 2) + (r & 3), s[r] * irs, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
           }
         }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          f32x8 ds;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) ds[r] = s[8 * k + r];
+          df[p][k] = El<TY>::frag(ds);
+        }
       }
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int p = 0; p < MAPS; ++p)
+#pragma unroll
+          for (int d = 0; d < DQ / 32; ++d) dq[p][d] = El<TY>::mma(TK::read_cols(kt + p * MB, 32 * u + 16 * k, d, lane), df[p][k], dq[p][d]);
     }
-    if (t + 1 < nt) put((t & 1) ^ 1);
+    dma_wait<0>();
     __syncthreads();
   }
 
@@ -285,8 +278,11 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
         }
   }
   if constexpr (BIAS) {
-    sum_l = wave_sum(sum_l);
-    sum_r = wave_sum(sum_r);
+    // A row's dS sums to zero, but for delta's error (it comes from an output that was rounded): of the far buckets, where P's
+    // sum is large, that error times the sum is taken off again.
+    const float e = half_sum((sum_l + sum_r) + sum_n);
+    sum_l = wave_sum(ok ? fmaf(-e, p_l, sum_l) : 0.0f);
+    sum_r = wave_sum(ok ? fmaf(-e, p_r, sum_r) : 0.0f);
     if (lane == 0) {                                  // the ends of the table stand for everything beyond
       hist[2 * wave * wk.nrel] += sum_l;
       hist[2 * wave * wk.nrel + wk.nrel - 1] += sum_r;
@@ -296,23 +292,36 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
       float v = 0.0f;
 #pragma unroll
       for (int c = 0; c < 8; ++c) v += hist[c * wk.nrel + i];
-      part[i] = v;
+      tab[i] = v;                                     // the bias itself is no longer needed
+    }
+    __syncthreads();
+    // by bucket: a run of distances each, first and count behind the table of buckets; the outermost reach to the table's ends
+    const int* run = a.lut + 2 * a.reach + 1;
+    for (int k = tid; k < a.num_buckets; k += 256) {
+      int i0 = run[k], i1 = i0 + run[a.num_buckets + k];
+      float v = 0.0f;
+      if (i1 > i0) {
+        i0 = i0 == 0 ? 0 : i0 + BIAS_PAD;
+        i1 = i1 == 2 * a.reach + 1 ? wk.nrel : i1 + BIAS_PAD;
+        for (int i = i0; i < i1; ++i) v += tab[i];
+      }
+      part[k] = v;
     }
   }
 }
 
 template <int TY, int MAPS, int DQ, int DV, bool BIAS>
-__global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnArgs a, int nblk) {
+__global__ __launch_bounds__(256, (MAPS * DQ + DV > 128 || (TY == TY_F32 && MAPS * DQ + DV > 64)) ? 1 : 2) void attn_dkv_kernel(AttnArgs a, int nblk) {
   typedef typename El<TY>::T T;
   typedef typename El<TY>::Frag Frag;
-  constexpr int QT = 32;
+  constexpr int QT = 64;
   typedef Tile<TY, DQ> TQ;
   typedef Tile<TY, DV> TG;
-  constexpr int QB = MAPS * QT * TQ::ROWB, GB = QT * TG::ROWB, SB = 3 * MAPS * QT * 4, ST = QB + GB + SB;
-  extern __shared__ __align__(16) char smem[];       // 2 x (Q maps, dO, statistics m | lg | delta of each map) | bias table
+  constexpr int MB = QT * TQ::ROWB, QB = MAPS * MB, GB = QT * TG::ROWB, SB = 4 * MAPS * QT * 4, ST = QB + GB + SB;
+  extern __shared__ __align__(16) char smem[];       // 2 x (Q maps, dO, per map and query: start, -delta, m, lg) | bias table
   const BwdWork wk(a, MAPS);
   float* tab = reinterpret_cast<float*>(smem + 2 * ST);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, half = lane >> 5;
   const int bh = blockIdx.x % (a.B * a.Hkv), b = bh / a.Hkv, hk = bh % a.Hkv, blk = blockIdx.x / (a.B * a.Hkv);
   const int G = a.H / a.Hkv;
   const int nq = clamp_len(a.q_len, b, a.Lq), nk = clamp_len(a.kv_len, b, a.Lk), st = start_of(a.q_start, b);
@@ -320,6 +329,44 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnArgs a, int nblk) 
   if (blk0 >= nk) return;
   const int key0 = blk0 + wave * 32, key = key0 + li;
   const bool ok = key < nk;
+  const float c2 = a.scale * LOG2E, ic2 = 1.0f / c2;
+  // under a causal mask the first query that sees key blk0 stands at its position
+  const int q_first = a.causal ? min(max(blk0 - st, 0), nq) / QT * QT : 0;
+  const int nt = nq > q_first ? (nq - q_first + QT - 1) / QT : 0;
+  const int wave_first = key0 >= nk ? 0x7fffffff : a.causal ? key0 - st : -0x7fffffff;    // first query that sees any of this wave's keys
+
+  Dma<TY, DQ, QT, 256> qd;
+  Dma<TY, DV, QT, 256> gd;
+  qd.init(a.sq[1], a.D, tid);
+  gd.init(a.sdo[1], a.Dv, tid);
+  float st_m = 0.0f, st_l = 0.0f, st_d = 0.0f;       // thread tid < MAPS QT: one query's statistics
+  auto fetch = [&](int h, int r0, int buf) {
+    char* base = smem + buf * ST;
+    const T* qp = (const T*)a.q + b * a.sq[0] + h * a.sq[2] + r0 * a.sq[1];
+#pragma unroll
+    for (int p = 0; p < MAPS; ++p) qd.issue(qp + (MAPS == 2 ? p * a.sq[3] : 0), nq - r0, base + p * MB, wave);
+    gd.issue((const T*)a.dout + b * a.sdo[0] + h * a.sdo[2] + r0 * a.sdo[1], nq - r0, base + QB, wave);
+    if (tid < MAPS * QT) {
+      const int p = tid / QT, row = r0 + tid % QT;
+      const long at = (((long)p * a.B + b) * a.H + h) * a.Lq + row;
+      const bool in = row < nq;                       // a query that is none: weights of exp2(-inf)
+      st_m = in ? a.stats[2 * at] : 0.0f;
+      st_l = in ? a.stats[2 * at + 1] : INFINITY;
+      st_d = in ? a.ws[wk.delta + at] : 0.0f;
+    }
+  };
+  auto put = [&](int buf) {
+    if (tid < MAPS * QT) {
+      float* d = reinterpret_cast<float*>(smem + buf * ST + QB + GB) + (tid / QT) * 4 * QT + tid % QT;
+      d[0] = (-st_m - st_l) * ic2;
+      d[QT] = -st_d;
+      d[2 * QT] = st_m;
+      d[3 * QT] = st_l;
+    }
+  };
+  const int steps = nt * G;
+  if (steps > 0) fetch(hk * G, q_first, 0);
+
   float lam = 0.0f;
   if constexpr (MAPS == 2) {
     float e1, e2;
@@ -352,124 +399,101 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnArgs a, int nblk) 
   }
   f32x16 dk[MAPS][DQ / 32], dv[DV / 32];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
+  for (int p = 0; p < MAPS; ++p)
 #pragma unroll
-    for (int p = 0; p < MAPS; ++p)
+    for (int d = 0; d < DQ / 32; ++d) dk[p][d] = zero16();
 #pragma unroll
-      for (int d = 0; d < DQ / 32; ++d) dk[p][d][r] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < DV / 32; ++d) dv[d][r] = 0.0f;
-  }
-  const float c2 = a.scale * LOG2E;
-  // under a causal mask the first query that sees key blk0 stands at its position
-  const int q_first = a.causal ? min(max(blk0 - st, 0), nq) / QT * QT : 0;
-  const int nt = nq > q_first ? (nq - q_first + QT - 1) / QT : 0;
-  const int wave_first = a.causal ? key0 - st : 0;    // first query that sees any of this wave's keys
+  for (int d = 0; d < DV / 32; ++d) dv[d] = zero16();
 
-  Stage<TY, DQ, QT, 256> qs[MAPS];
-  Stage<TY, DV, QT, 256> gs;
-  float sv = 0.0f;                                    // thread tid < 3 MAPS QT: one statistic of the tile
-  auto fetch = [&](int it) {
-    const int h = hk * G + it / nt, r0 = q_first + it % nt * QT;
-    const T* qp = (const T*)a.q + b * a.sq[0] + h * a.sq[2];
-    const T* gp = (const T*)a.dout + b * a.sdo[0] + h * a.sdo[2];
-#pragma unroll
-    for (int p = 0; p < MAPS; ++p) qs[p].load(qp + (MAPS == 2 ? p * a.sq[3] : 0), a.sq[1], r0, nq, a.D, tid);
-    gs.load(gp, a.sdo[1], r0, nq, a.Dv, tid);
-    if (tid < 3 * MAPS * QT) {
-      const int what = tid / QT, p = what / 3, kind = what % 3, row = r0 + tid % QT;
-      const long at = (((long)p * a.B + b) * a.H + h) * a.Lq + row;
-      // a row that is none: weights of exp2(-inf)
-      sv = row >= nq ? (kind == 1 ? INFINITY : 0.0f) : kind == 2 ? a.ws[wk.delta + at] : a.stats[2 * at + kind];
-    }
-  };
-  auto put = [&](int buf) {
-    char* base = smem + buf * ST;
-#pragma unroll
-    for (int p = 0; p < MAPS; ++p) qs[p].store(base + p * QT * TQ::ROWB, tid);
-    gs.store(base + QB, tid);
-    if (tid < 3 * MAPS * QT) reinterpret_cast<float*>(base + QB + GB)[tid] = sv;
-  };
-  const int steps = nt * G;
-  int filled = -1;
-  if (steps > 0) {
-    fetch(0);
-    put(0);
-  }
   float far_l = 0.0f, far_r = 0.0f;
   bool fold = true;
+  int h = hk * G, r0 = q_first;
+  if (steps > 0) put(0);
   for (int it = 0; it < steps; ++it) {
-    const int h = hk * G + it / nt, r0 = q_first + it % nt * QT;
-    if (BIAS && filled != h) {
-      // every wave is past its last read of the table: the barrier at the end of the step before
+    if (BIAS && r0 == q_first) {
+      // a new head: every wave is past its last read of the old one's table, by the barrier at the end of the step before
       fill_bias<TY>(a, tab, h, tid, 256);
       far_l = bias_log2<TY>(a, -a.reach, h);
       far_r = bias_log2<TY>(a, a.reach, h);
       fold = fabsf(far_l) < BIAS_FOLD && fabsf(far_r) < BIAS_FOLD;
-      filled = h;
     }
-    if (it == 0 || (BIAS && it % nt == 0)) __syncthreads();
+    if (it == 0) dma_wait<0>();
+    if (it == 0 || (BIAS && r0 == q_first)) __syncthreads();
     const char* qt = smem + (it & 1) * ST;
     const char* gt = qt + QB;
     const float* stat = reinterpret_cast<const float*>(gt + GB);
-    if (it + 1 < steps) fetch(it + 1);
-    if (key0 < nk && r0 + QT - 1 >= wave_first) {
-      f32x16 x;
+    int hn = h, rn = r0 + QT;
+    if (rn >= nq) {
+      hn = h + 1;
+      rn = q_first;
+    }
+    if (it + 1 < steps) fetch(hn, rn, (it & 1) ^ 1);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = 0.0f;
+    for (int u = 0; u < QT / 32; ++u) {
+      const int q0 = r0 + 32 * u;
+      if (q0 + 31 < wave_first || q0 >= nq) continue;
+      const bool diag = a.causal && q0 < key0 + 31 - st;             // some pair of the tile is masked
+      const bool left = BIAS && key0 + 31 - (st + q0) <= -a.reach, right = BIAS && key0 - (st + q0 + 31) >= a.reach;
+      const bool plain = !diag && (!BIAS || (fold && (left || right)));
+      // register row 8 c + 4 half + r, c = 0..3: its statistics in four 16-byte pieces, the same for all lanes of a half
+      auto rows16 = [&](int p, int what) {
+        f32x16 v;
 #pragma unroll
-      for (int k = 0; k < DV / 16; ++k) x = El<TY>::mma(TG::read_rows(gt, li, k, half), vf[k], x);
-      const bool diag = a.causal && r0 < key0 + 31 - st;             // some pair of the tile is masked
-      const int first = key - st - r0 - 4 * half;                    // register rows from here on see this lane's key
+        for (int c = 0; c < 4; ++c) {
+          const f32x4 t = *reinterpret_cast<const f32x4*>(stat + (4 * p + what) * QT + 32 * u + 8 * c + 4 * half);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[4 * c + r] = t[r];
+        }
+        return v;
+      };
+      f32x16 x = rows16(0, 1);                                       // X - delta: the product starts from -delta
+#pragma unroll
+      for (int k = 0; k < DV / 16; ++k) x = El<TY>::mma(TG::read_rows(gt, 32 * u + li, k, half), vf[k], x);
       f32x16 w0;
       Frag dsf[MAPS][2];
 #pragma unroll
       for (int p = 0; p < MAPS; ++p) {
-        f32x16 s;
+        f32x16 s = zero16();
+        if (plain) s = rows16(p, 0);                                 // and the exponent from (-m - lg) / c2
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+        for (int k = 0; k < DQ / 16; ++k) s = El<TY>::mma(TQ::read_rows(qt + p * MB, 32 * u + li, k, half), kf[p][k], s);
+        if (plain) {
+          const float far = !BIAS ? 0.0f : left ? far_l : far_r;
 #pragma unroll
-        for (int k = 0; k < DQ / 16; ++k) s = El<TY>::mma(TQ::read_rows(qt + p * QT * TQ::ROWB, li, k, half), kf[p][k], s);
-        bool left = false, right = false;
-        if constexpr (BIAS) {
-          left = key0 + 31 - (st + r0) <= -a.reach;
-          right = key0 - (st + r0 + QT - 1) >= a.reach;
-        }
-        const float* tp = tab + a.reach + BIAS_PAD + (key - st - r0 - 4 * half);
-        const float far = left ? far_l : far_r;
+          for (int r = 0; r < 16; ++r) s[r] = exp2_(BIAS ? fmaf(s[r], c2, far) : s[r] * c2);
+        } else {
+          const f32x16 mm = rows16(p, 2), ll = rows16(p, 3);
+          const int first = diag ? key - st - q0 - 4 * half : -64;   // register rows from here on see this lane's key
+          const float* tp = tab + a.reach + BIAS_PAD + (key - st - q0 - 4 * half);
+          const bool near = BIAS && !left && !right;
+          const float far = left ? far_l : far_r;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const f32x4 m4 = *reinterpret_cast<const f32x4*>(stat + (3 * p) * QT + 8 * c + 4 * half);
-          const f32x4 l4 = *reinterpret_cast<const f32x4*>(stat + (3 * p + 1) * QT + 8 * c + 4 * half);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float e;
-            if (!BIAS) e = fmaf(s[4 * c + r], c2, -m4[r] - l4[r]);
-            else if ((left || right) && fold) e = fmaf(s[4 * c + r], c2, (far - m4[r]) - l4[r]);
-            else e = (fmaf(s[4 * c + r], c2, (left || right) ? far : tp[-(8 * c + r)]) - m4[r]) - l4[r];
-            if (diag) e = 8 * c + r >= first ? e : -INFINITY;
-            s[4 * c + r] = exp2_(e);
+          for (int r = 0; r < 16; ++r) {
+            const int c = 8 * (r >> 2) + (r & 3);
+            const float e = (fmaf(s[r], c2, !BIAS ? 0.0f : near ? tp[-c] : far) - mm[r]) - ll[r];
+            s[r] = c >= first ? exp2_(e) : 0.0f;
           }
         }
-        // P (for dV) and dS
         if (MAPS == 2 && p == 1) {
+          // the second map weighs -lambda, and its delta is its own
+          const f32x16 d0 = rows16(0, 1), d1 = rows16(1, 1);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] *= -lam;
-        }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) w0[r] = p == 0 ? s[r] : w0[r] + s[r];
-        f32x16 ds;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const f32x4 d4 = *reinterpret_cast<const f32x4*>(stat + (3 * p + 2) * QT + 8 * c + 4 * half);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) ds[4 * c + r] = s[4 * c + r] * (TY == TY_F16 ? fmaf(x[4 * c + r], rs, -d4[r] * rs) : x[4 * c + r] - d4[r]);
+          for (int r = 0; r < 16; ++r) {
+            s[r] *= -lam;
+            w0[r] += s[r];
+            x[r] += d1[r] - d0[r];
+          }
+        } else {
+          w0 = s;
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           f32x8 t;
 #pragma unroll
-          for (int r = 0; r < 8; ++r) t[r] = ds[8 * k + r];
+          for (int r = 0; r < 8; ++r) {
+            t[r] = s[8 * k + r] * x[8 * k + r];
+            if (TY == TY_F16) t[r] *= rs;
+          }
           dsf[p][k] = El<TY>::frag(t);
         }
       }
@@ -480,14 +504,17 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnArgs a, int nblk) 
         for (int r = 0; r < 8; ++r) t[r] = w0[8 * k + r];
         const Frag pf = El<TY>::frag(t);
 #pragma unroll
-        for (int d = 0; d < DV / 32; ++d) dv[d] = El<TY>::mma(TG::read_cols(gt, 16 * k, d, lane), pf, dv[d]);
+        for (int d = 0; d < DV / 32; ++d) dv[d] = El<TY>::mma(TG::read_cols(gt, 32 * u + 16 * k, d, lane), pf, dv[d]);
 #pragma unroll
         for (int p = 0; p < MAPS; ++p)
 #pragma unroll
-          for (int d = 0; d < DQ / 32; ++d) dk[p][d] = El<TY>::mma(TQ::read_cols(qt + p * QT * TQ::ROWB, 16 * k, d, lane), dsf[p][k], dk[p][d]);
+          for (int d = 0; d < DQ / 32; ++d) dk[p][d] = El<TY>::mma(TQ::read_cols(qt + p * MB, 32 * u + 16 * k, d, lane), dsf[p][k], dk[p][d]);
       }
     }
+    h = hn;
+    r0 = rn;
     if (it + 1 < steps) put((it & 1) ^ 1);
+    dma_wait<0>();
     __syncthreads();
   }
   if (!ok) return;
@@ -513,32 +540,22 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(AttnArgs a, int nblk) 
   }
 }
 
-// One work-group a head: sums by distance over samples and query blocks, then by bucket.
+// A work-group a head and bucket: sums over samples and query blocks, in a fixed order.
 template <int TY>
-__global__ __launch_bounds__(1024) void rel_dw_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256) void rel_dw_kernel(AttnArgs a) {
   typedef typename El<TY>::T T;
   const BwdWork wk(a, 1);
-  __shared__ float by[2 * (1024 + BIAS_PAD) + 1];
-  const int h = blockIdx.x, tid = threadIdx.x;
-  for (int i = tid; i < wk.nrel; i += 1024) {
-    float v = 0.0f;
-    for (int b = 0; b < a.B; ++b) {
-      const float* p = a.ws + wk.part + ((long)(b * a.H + h) * wk.nblk) * wk.nrel + i;
-      float t = 0.0f;
-      for (int c = 0; c < wk.nblk; ++c) t += p[(long)c * wk.nrel];
-      v += t;
-    }
-    by[i] = v;
+  __shared__ float red[4];
+  const int k = blockIdx.x % a.num_buckets, h = blockIdx.x / a.num_buckets, tid = threadIdx.x;
+  float v = 0.0f;
+  for (int i = tid; i < a.B * wk.nblk; i += 256) {
+    const int b = i / wk.nblk, c = i % wk.nblk;
+    v += a.ws[wk.part + ((long)(b * a.H + h) * wk.nblk + c) * wk.nsum + k];
   }
+  v = wave_sum(v);
+  if ((tid & 63) == 0) red[tid >> 6] = v;
   __syncthreads();
-  for (int k = tid; k < a.num_buckets; k += 1024) {
-    float v = 0.0f;
-    for (int i = 0; i < wk.nrel; ++i) {
-      const int rel = min(max(i - a.reach - BIAS_PAD, -a.reach), a.reach);
-      if (a.lut[rel + a.reach] == k) v += by[i];
-    }
-    El<TY>::store((T*)a.dw + (long)k * a.H + h, v);
-  }
+  if (tid == 0) El<TY>::store((T*)a.dw + (long)k * a.H + h, (red[0] + red[1]) + (red[2] + red[3]));
 }
 
 // dlambda over all work-groups, then the four vectors
@@ -577,11 +594,11 @@ template <int TY, int MAPS, int DQ, int DV, bool BIAS> static int launch_bwd(con
   hipLaunchKernelGGL((attn_dq_kernel<TY, MAPS, DQ, DV, BIAS>), dim3(a->B * a->H * wk.nblk), dim3(256), lds, stream, *a);
   SGTA_LAUNCH_CHECK();
   const int nblk = cdiv(a->Lk, 128);
-  lds = 2 * (32 * (MAPS * DQ + DV) * SZ + 3 * MAPS * 32 * 4) + tab;
+  lds = 2 * (64 * (MAPS * DQ + DV) * SZ + 4 * MAPS * 64 * 4) + tab;
   if (int e = allow_lds<attn_dkv_kernel<TY, MAPS, DQ, DV, BIAS>>(lds)) return e;
   hipLaunchKernelGGL((attn_dkv_kernel<TY, MAPS, DQ, DV, BIAS>), dim3(a->B * a->Hkv * nblk), dim3(256), lds, stream, *a, nblk);
   SGTA_LAUNCH_CHECK();
-  if (MAPS == 1) hipLaunchKernelGGL((rel_dw_kernel<TY>), dim3(a->H), dim3(1024), 0, stream, *a);
+  if (MAPS == 1) hipLaunchKernelGGL((rel_dw_kernel<TY>), dim3(a->H * a->num_buckets), dim3(256), 0, stream, *a);
   else hipLaunchKernelGGL((diff_dw_kernel<TY>), dim3(1), dim3(256), 0, stream, *a);
   SGTA_LAUNCH_CHECK();
   return SGTA_OK;
@@ -594,6 +611,7 @@ static int bwd_check(const AttnArgs* a, int maps) {
   const int al = a->dtype == TY_F32 ? 4 : 8;
   const long* s[] = {a->sdo, a->sdq, a->sdk, a->sdv};
   const void* p[] = {a->dout, a->dq, a->dk, a->dv};
+  if (a->sdo[1] < 0 || a->sdo[1] > MAX_PITCH / (a->dtype == TY_F32 ? 4 : 2)) return SGTA_ETOOBIG;
   for (int i = 0; i < 4; ++i) {
     if ((uintptr_t)p[i] % 16) return SGTA_EBADARG;
     for (int j = 0; j < ((i == 1 || i == 2) && maps == 2 ? 4 : 3); ++j)

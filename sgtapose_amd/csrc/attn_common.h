@@ -122,30 +122,54 @@ template <int TY, int COLS> struct Tile {
   }
 };
 
-// Rows [row0, row0 + ROWS) of a strided matrix on their way into a Tile: global loads into registers now, LDS stores later.
-// Rows from ``rows`` on and elements from ``cols`` on are zero and never read: what lies there may be anything.
-template <int TY, int COLS, int ROWS, int NT> struct Stage {
+// Global memory -> LDS, 16 bytes a lane, to LDS byte ``at`` + 16 lane.  In assembly although there is a builtin: of that the
+// compiler assumes that any transposing LDS read may see its data, and waits for all of it (the NEXT tile) before each of them.
+// It has no result register; what was loaded is read only after dma_wait and a barrier.
+#if defined(__HIP_DEVICE_COMPILE__)
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, unsigned off, unsigned at) {
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(rs) : "memory", "m0");
+}
+#endif
+
+// Rows of a strided matrix into a Tile by NT threads, straight into LDS (no registers, no LDS store instructions): a wave writes
+// 64 consecutive pieces, so each lane fetches the piece that belongs at its place of the swizzle.  Rows from ``rows`` on and
+// elements from ``cols`` on are zero and never read: what lies there may be anything.  The loads are in flight until dma_wait.
+template <int TY, int COLS, int ROWS, int NT> struct Dma {
   typedef Tile<TY, COLS> Tl;
   typedef typename El<TY>::T T;
   static constexpr int ALL = ROWS * Tl::CH, N = (ALL + NT - 1) / NT;
-  u32x4 r[N];
-  __device__ __forceinline__ void load(const T* p, long ld, int row0, int rows, int cols, int tid) {
+  static_assert(ALL % 64 == 0, "whole waves");
+  unsigned off[N];
+  int pitch, tail;                                    // bytes from row to row; bytes of a row
+  __device__ __forceinline__ void init(long ld, int cols, int tid) {
+    pitch = (int)ld * Tl::SZ;                         // at most MAX_PITCH: checked at the entry points
+    tail = cols * Tl::SZ;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int c = tid + i * NT, row = row0 + c / Tl::CH, e = (c % Tl::CH) * Tl::EPC;
-      u32x4 z = {0, 0, 0, 0};
-      r[i] = z;
-      if ((ALL % NT == 0 || c < ALL) && row < rows && e < cols) r[i] = *reinterpret_cast<const u32x4*>(p + (long)row * ld + e);
+      const int p = tid + i * NT, row = p / Tl::CH, ch = (p % Tl::CH) ^ Tl::swz(row);
+      off[i] = ch * 16 < tail ? (unsigned)(row * pitch + ch * 16) : 0x80000000u;
     }
   }
-  __device__ __forceinline__ void store(char* lds, int tid) const {
+  // p: the tile's first row; rows: valid rows from there on; wave: this thread's wave of the NT / 64
+  __device__ __forceinline__ void issue(const T* p, int rows, char* lds, int wave) const {
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef __attribute__((address_space(3))) void* lds_ptr_t;
+    const int n = min(rows, ROWS);
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), (short)0, n > 0 ? (n - 1) * pitch + tail : 0, 0x00020000);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = tid + i * NT;
-      if (ALL % NT == 0 || c < ALL) *reinterpret_cast<u32x4*>(lds + Tl::piece(c / Tl::CH, c % Tl::CH)) = r[i];
-    }
+    for (int i = 0; i < N; ++i)
+      if (ALL % NT == 0 || i * NT + wave * 64 < ALL) dma16(rs, off[i], (unsigned)(size_t)(lds_ptr_t)(lds + (i * NT + wave * 64) * 16));
+#endif
   }
 };
+#define MAX_PITCH (1 << 24)
+// until at most KEEP of this wave's loads are in flight
+template <int KEEP> __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(KEEP) : "memory"); }
+
+__device__ __forceinline__ f32x16 zero16() {
+  const f32x16 z = {0};
+  return z;
+}
 
 // eight consecutive elements of a global row as an operand fragment (zero where ``ok`` is false)
 template <int TY> __device__ __forceinline__ typename El<TY>::Frag global_frag(const typename El<TY>::T* p, bool ok) {

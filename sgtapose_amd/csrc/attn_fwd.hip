@@ -13,18 +13,20 @@
 #include "attn_common.h"
 
 // One wave's 32 query rows: fragments, running statistics, the accumulated O^T.
-template <int TY, int MAPS, int DQ, int DV, bool BIAS, int KT> struct FwdWave {
+template <int TY, int MAPS, int DQ, int DV, bool BIAS> struct FwdWave {
   typedef typename El<TY>::T T;
   typedef typename El<TY>::Frag Frag;
-  static constexpr int NS = KT / 32;
+  typedef Tile<TY, DQ> TK;
+  typedef Tile<TY, DV> TV;
   Frag q[MAPS][DQ / 16];
   f32x16 o[MAPS][DV / 32];
   float m[MAPS], l[MAPS];      // running reference (log2 units) and this lane half's part of the sum
-  int limit;                   // last key this lane's query sees (-1: none)
+  int limit, low;              // last key this lane's query sees; the least of the wave's
   int pos, pmin, pmax;         // the lane's position; the wave's first and last
   const float* tab;            // BIAS: this lane's head's table, at rel = 0
   float far_l, far_r;          // its values left and right of ``reach``
   bool fold;                   // both may be folded into the exponent
+  float c2;                    // scale in log2 units
 
   __device__ __forceinline__ void init() {
 #pragma unroll
@@ -32,9 +34,7 @@ template <int TY, int MAPS, int DQ, int DV, bool BIAS, int KT> struct FwdWave {
       m[p] = -INFINITY;
       l[p] = 0.0f;
 #pragma unroll
-      for (int d = 0; d < DV / 32; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[p][d][r] = 0.0f;
+      for (int d = 0; d < DV / 32; ++d) o[p][d] = zero16();
     }
   }
 
@@ -48,91 +48,90 @@ template <int TY, int MAPS, int DQ, int DV, bool BIAS, int KT> struct FwdWave {
       }
   }
 
-  // keys [j0, j0 + KT) from LDS; rows of kt beyond the last key are zero
-  __device__ __forceinline__ void tile(const char* kt, const char* vt, int j0, int reach, float c2, int lane) {
-    typedef Tile<TY, DQ> TK;
-    typedef Tile<TY, DV> TV;
+  // Scores of NK keys -> weights, in place; returns by how much the accumulators shrink.  cc, add: what is left to apply to them.
+  template <int NS> __device__ __forceinline__ float weights(f32x16 (&s)[NS], int p, float cc, float add, bool& grown) {
+    float mx = s[0][0];
+#pragma unroll
+    for (int u = 0; u < NS; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[u][r]);
+    mx = fmaf(half_max(mx), cc, add);
+    // the reference follows the maximum only where that has grown by more than 2^8: weights stay below 2^8, far inside every
+    // type's range, and most tiles leave the accumulators alone
+    grown = mx > m[p] + 8.0f;
+    const float mn = grown ? mx : m[p];
+    const float al = grown ? exp2_(m[p] - mn) : 1.0f;
+    m[p] = mn;
+    const float sub = add - (mn == -INFINITY ? 0.0f : mn);
+    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int u = 0; u < NS; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[u][r] = exp2_(fmaf(s[u][r], cc, sub));
+        part[r & 3] += s[u][r];
+      }
+    l[p] = fmaf(l[p], al, (part[0] + part[1]) + (part[2] + part[3]));
+    return al;
+  }
+
+  // NK keys from j0 on, which are rows k0 ... of the LDS tiles (maps ``mapb`` bytes apart)
+  template <int NK> __device__ __forceinline__ void step(const char* kt, int mapb, const char* vt, int k0, int j0, int reach, int lane) {
+    constexpr int NS = NK / 32;
     const int li = lane & 31, half = lane >> 5;
-    const bool masked = __any(limit < j0 + KT - 1);
-    Frag pf[MAPS][KT / 16];
+    const bool masked = low < j0 + NK - 1;
+    const bool left = BIAS && j0 + NK - 1 - pmin <= -reach, right = BIAS && j0 - pmax >= reach;
+    // plain: every query sees every key and the bias is one value, which goes into the exponent
+    const bool plain = !masked && (!BIAS || (fold && (left || right)));
+    Frag pf[MAPS][NK / 16];
 #pragma unroll
     for (int p = 0; p < MAPS; ++p) {
       f32x16 s[NS];
 #pragma unroll
       for (int u = 0; u < NS; ++u) {
+        s[u] = zero16();
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[u][r] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < DQ / 16; ++k)
-          s[u] = El<TY>::mma(TK::read_rows(kt + p * KT * TK::ROWB, 32 * u + li, k, half), q[p][k], s[u]);
+        for (int k = 0; k < DQ / 16; ++k) s[u] = El<TY>::mma(TK::read_rows(kt + p * mapb, k0 + 32 * u + li, k, half), q[p][k], s[u]);
       }
-      float cc = c2, add = 0.0f;
-      if constexpr (BIAS) {
-        const bool left = j0 + KT - 1 - pmin <= -reach, right = j0 - pmax >= reach;
-        if (fold && (left || right)) {
-          add = left ? far_l : far_r;
-        } else if (left || right) {
-          const float b = left ? far_l : far_r;
-          cc = 1.0f;
-#pragma unroll
-          for (int u = 0; u < NS; ++u)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[u][r] = fmaf(s[u][r], c2, b);
-        } else {
-          const float* t = tab + (j0 + 4 * half - pos);
-          cc = 1.0f;
-#pragma unroll
-          for (int u = 0; u < NS; ++u)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[u][r] = fmaf(s[u][r], c2, t[32 * u + 8 * (r >> 2) + (r & 3)]);
-        }
-      }
-      if (masked) {
-        const int last = limit - j0 - 4 * half;
+      float al;
+      bool grown;
+      if (plain) {
+        al = weights<NS>(s, p, c2, !BIAS ? 0.0f : left ? far_l : far_r, grown);
+      } else {
+        const int last = masked ? limit - j0 - 4 * half : NK;
+        const float far = left ? far_l : far_r;
+        const float* t = tab + (j0 + 4 * half - pos);
+        const bool near = BIAS && !left && !right;
 #pragma unroll
         for (int u = 0; u < NS; ++u)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[u][r] = 32 * u + 8 * (r >> 2) + (r & 3) <= last ? s[u][r] : -INFINITY;
+          for (int r = 0; r < 16; ++r) {
+            const int c = 32 * u + 8 * (r >> 2) + (r & 3);
+            float x = s[u][r] * c2;
+            if (BIAS) x = fmaf(s[u][r], c2, near ? t[c] : far);
+            s[u][r] = c <= last ? x : -INFINITY;
+          }
+        al = weights<NS>(s, p, 1.0f, 0.0f, grown);
       }
-      float mx = s[0][0];
+      if (__any(grown)) {
 #pragma unroll
-      for (int u = 0; u < NS; ++u)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[u][r]);
-      mx = fmaf(half_max(mx), cc, add);
-      // the reference follows the maximum only where that has grown by more than 2^8: weights stay below 2^8, far inside
-      // every type's range, and most tiles leave the accumulators alone
-      if (__any(mx > m[p] + 8.0f)) {
-        const float mn = fmaxf(m[p], mx);
-        const float al = mn == -INFINITY ? 1.0f : exp2_(m[p] - mn);
-        m[p] = mn;
-        l[p] *= al;
-#pragma unroll
-        for (int d = 0; d < DV / 32; ++d)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[p][d][r] *= al;
+        for (int d = 0; d < DV / 32; ++d) o[p][d] *= al;
       }
-      const float sub = add - (m[p] == -INFINITY ? 0.0f : m[p]);
-      float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int u = 0; u < NS; ++u)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           f32x8 e;
 #pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            e[r] = exp2_(fmaf(s[u][8 * t + r], cc, sub));
-            part[r & 3] += e[r];
-          }
+          for (int r = 0; r < 8; ++r) e[r] = s[u][8 * t + r];
           pf[p][2 * u + t] = El<TY>::frag(e);
         }
-      l[p] += (part[0] + part[1]) + (part[2] + part[3]);
     }
 #pragma unroll
-    for (int t = 0; t < KT / 16; ++t)
+    for (int t = 0; t < NK / 16; ++t)
 #pragma unroll
       for (int d = 0; d < DV / 32; ++d) {
-        const Frag vf = TV::read_cols(vt, 16 * t, d, lane);
+        const Frag vf = TV::read_cols(vt, k0 + 16 * t, d, lane);
 #pragma unroll
         for (int p = 0; p < MAPS; ++p) o[p][d] = El<TY>::mma(vf, pf[p][t], o[p][d]);
       }
@@ -169,28 +168,45 @@ __device__ __forceinline__ FwdPlace fwd_place(const AttnArgs& a, int nblk) {
 template <int TY, int MAPS, int DQ, int DV, bool BIAS>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a, int nblk) {
   typedef typename El<TY>::T T;
-  constexpr int KT = TY == TY_F32 ? 32 : 64;
-  typedef Tile<TY, DQ> TK;
-  typedef Tile<TY, DV> TV;
-  constexpr int KB = MAPS * KT * TK::ROWB, VB = KT * TV::ROWB;
+  constexpr int KT = TY == TY_F32 ? 32 : 64, NK = TY == TY_F32 || (MAPS == 2 && DV > 64) ? 32 : 64;   // keys staged; keys at a time
+  constexpr int MB = KT * DQ * (int)sizeof(T), KB = MAPS * MB, VB = KT * DV * (int)sizeof(T);
   extern __shared__ __align__(16) char smem[];       // 2 x (K maps, V), then the bias table
   float* tab = reinterpret_cast<float*>(smem + 2 * (KB + VB));
   const FwdPlace w = fwd_place(a, nblk);
   if (!w.ok) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, half = lane >> 5;
   const int b = w.b, h = w.h, hk = h / (a.H / a.Hkv);
   const int nq = clamp_len(a.q_len, b, a.Lq), nk = clamp_len(a.kv_len, b, a.Lk), st = start_of(a.q_start, b);
   const int blk0 = w.blk * 128;
   if (blk0 >= nq) return;
   const int row0 = blk0 + wave * 32, row = row0 + li;
+  const int last_row = min(blk0 + 127, nq - 1);
+  const int seen = a.causal ? min(nk, max(st + last_row + 1, 0)) : nk;      // keys any row of this block sees
+  const int nt = (seen + KT - 1) / KT;
 
-  FwdWave<TY, MAPS, DQ, DV, BIAS, KT> wv;
+  const T* kp = (const T*)a.k + b * a.sk[0] + hk * a.sk[2];
+  const T* vp = (const T*)a.v + b * a.sv[0] + hk * a.sv[2];
+  Dma<TY, DQ, KT, 256> kd;
+  Dma<TY, DV, KT, 256> vd;
+  kd.init(a.sk[1], a.D, tid);
+  vd.init(a.sv[1], a.Dv, tid);
+  auto fetch = [&](int j0, int buf) {
+    char* base = smem + buf * (KB + VB);
+#pragma unroll
+    for (int p = 0; p < MAPS; ++p) kd.issue(kp + (MAPS == 2 ? p * a.sk[3] : 0) + j0 * a.sk[1], seen - j0, base + p * MB, wave);
+    vd.issue(vp + j0 * a.sv[1], seen - j0, base + KB, wave);
+  };
+  if (nt > 0) fetch(0, 0);
+
+  FwdWave<TY, MAPS, DQ, DV, BIAS> wv;
   wv.init();
   wv.load_q(a, (const T*)a.q + b * a.sq[0] + row * a.sq[1] + h * a.sq[2], row < nq, half);
   wv.pos = st + row;
   wv.pmin = st + row0;
   wv.pmax = st + row0 + 31;
-  wv.limit = row < nq ? min(nk - 1, a.causal ? wv.pos : nk - 1) : -1;
+  wv.limit = min(nk - 1, a.causal ? wv.pos : nk - 1);                // rows behind the last query: computed, not stored
+  wv.low = min(nk - 1, a.causal ? wv.pmin : nk - 1);
+  wv.c2 = a.scale * LOG2E;
   if constexpr (BIAS) {
     fill_bias<TY>(a, tab, h, tid, 256);
     wv.tab = tab + a.reach + BIAS_PAD;
@@ -198,38 +214,17 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a, int nblk) 
     wv.far_r = bias_log2<TY>(a, a.reach, h);
     wv.fold = fabsf(wv.far_l) < BIAS_FOLD && fabsf(wv.far_r) < BIAS_FOLD;
   }
-  const float c2 = a.scale * LOG2E;
-  const int last_row = min(blk0 + 127, nq - 1);
-  const int seen = a.causal ? min(nk, max(st + last_row + 1, 0)) : nk;      // keys any row of this block sees
-  const int nt = (seen + KT - 1) / KT;
-  const int wave_last = a.causal ? min(seen - 1, st + min(row0 + 31, nq - 1)) : seen - 1;
-  const bool active = row0 < nq;
+  const int wave_last = row0 >= nq ? -1 : a.causal ? min(seen - 1, st + min(row0 + 31, nq - 1)) : seen - 1;
 
-  const T* kp = (const T*)a.k + b * a.sk[0] + hk * a.sk[2];
-  const T* vp = (const T*)a.v + b * a.sv[0] + hk * a.sv[2];
-  Stage<TY, DQ, KT, 256> ks[MAPS];
-  Stage<TY, DV, KT, 256> vs;
-  auto fetch = [&](int j0) {
-#pragma unroll
-    for (int p = 0; p < MAPS; ++p) ks[p].load(kp + (MAPS == 2 ? p * a.sk[3] : 0), a.sk[1], j0, seen, a.D, tid);
-    vs.load(vp, a.sv[1], j0, seen, a.Dv, tid);
-  };
-  auto put = [&](int buf) {
-    char* base = smem + buf * (KB + VB);
-#pragma unroll
-    for (int p = 0; p < MAPS; ++p) ks[p].store(base + p * KT * TK::ROWB, tid);
-    vs.store(base + KB, tid);
-  };
-  if (nt > 0) {
-    fetch(0);
-    put(0);
-  }
+  dma_wait<0>();
   __syncthreads();
   for (int t = 0; t < nt; ++t) {
-    const int cur = t & 1;
-    if (t + 1 < nt) fetch((t + 1) * KT);
-    if (active && t * KT <= wave_last) wv.tile(smem + cur * (KB + VB), smem + cur * (KB + VB) + KB, t * KT, a.reach, c2, lane);
-    if (t + 1 < nt) put(cur ^ 1);
+    const char* kt = smem + (t & 1) * (KB + VB);
+    if (t + 1 < nt) fetch((t + 1) * KT, (t & 1) ^ 1);
+#pragma unroll
+    for (int u = 0; u < KT / NK; ++u)
+      if (t * KT + u * NK <= wave_last) wv.template step<NK>(kt, MB, kt + KB, u * NK, t * KT + u * NK, a.reach, lane);
+    dma_wait<0>();
     __syncthreads();
   }
 
@@ -277,64 +272,80 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a, int nblk) 
 // ---- few queries ---------------------------------------------------------------------------------
 // Rows r = i G + g of one (b, key / value head): query i, head hk G + g; R = Lq G <= 32.  ``splits`` work-groups share the
 // keys; part s of them leaves per map and row {m, l, O[0..DV)} in ws[((s B + b) Hkv + hk) ...], joined by attn_join_kernel.
+template <int TY, int MAPS, int DQ, int DV> struct StepTile {
+  static constexpr int SZ = sizeof(typename El<TY>::T), MB = 32 * DQ * SZ, KB = MAPS * MB, VB = 32 * DV * SZ;
+  static constexpr int BUFS = 8 * (KB + VB) <= 128 * 1024 ? 2 : 1;     // private tiles of a wave: the next is fetched over the present
+  static constexpr int REC = DV + 4;                                   // a row's part: O, m, l (padded to 16 bytes)
+  static constexpr int LDS = 4 * BUFS * (KB + VB), JOIN = 4 * 32 * REC * 4;
+};
+
 template <int TY, int MAPS, int DQ, int DV, bool BIAS>
 __global__ __launch_bounds__(256) void attn_step_kernel(AttnArgs a, int splits) {
   typedef typename El<TY>::T T;
-  constexpr int KT = 32;
-  typedef Tile<TY, DQ> TK;
-  typedef Tile<TY, DV> TV;
-  constexpr int KB = MAPS * KT * TK::ROWB, VB = KT * TV::ROWB;
-  constexpr int REC = DV + 4;                          // a row's part: O, m, l (padded to 16 bytes)
-  extern __shared__ __align__(16) char smem[];         // 4 x (K maps, V) private tiles | bias tables of the G heads
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, half = lane >> 5;
+  typedef StepTile<TY, MAPS, DQ, DV> L;
+  constexpr int KT = 32, REC = L::REC;
+  extern __shared__ __align__(16) char smem[];         // 4 waves x BUFS x (K maps, V) | bias tables of the G heads
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, half = lane >> 5;
   const int bh = blockIdx.x / splits, sp = blockIdx.x % splits, b = bh / a.Hkv, hk = bh % a.Hkv;
   const int G = a.H / a.Hkv, R = a.Lq * G;
   const int nq = clamp_len(a.q_len, b, a.Lq), nk = clamp_len(a.kv_len, b, a.Lk), st = start_of(a.q_start, b);
   const int row = li, i = row / G, g = row % G, h = hk * G + (row < R ? g : 0);
   const bool ok = row < R && i < nq;
-  char* mine = smem + wave * (KB + VB);
-  float* tabs = reinterpret_cast<float*>(smem + 4 * (KB + VB));
+  char* mine = smem + wave * L::BUFS * (L::KB + L::VB);
+  float* tabs = reinterpret_cast<float*>(smem + L::LDS);
 
-  FwdWave<TY, MAPS, DQ, DV, BIAS, KT> wv;
+  // each part ends where the next begins
+  const int seen = a.causal ? min(nk, max(st + nq, 0)) : nk;
+  const int per = ((seen + splits - 1) / splits + 127) / 128 * 128;      // keys per part: whole rounds of the 4 waves
+  const int k0 = min(sp * per, seen), k1 = min(k0 + per, seen);
+  const T* kp = (const T*)a.k + b * a.sk[0] + hk * a.sk[2];
+  const T* vp = (const T*)a.v + b * a.sv[0] + hk * a.sv[2];
+  Dma<TY, DQ, KT, 64> kd;
+  Dma<TY, DV, KT, 64> vd;
+  kd.init(a.sk[1], a.D, lane);
+  vd.init(a.sv[1], a.Dv, lane);
+  auto fetch = [&](int j0, char* base) {
+#pragma unroll
+    for (int p = 0; p < MAPS; ++p) kd.issue(kp + (MAPS == 2 ? p * a.sk[3] : 0) + j0 * a.sk[1], k1 - j0, base + p * L::MB, 0);
+    vd.issue(vp + j0 * a.sv[1], k1 - j0, base + L::KB, 0);
+  };
+  constexpr int LOADS = MAPS * Dma<TY, DQ, KT, 64>::N + Dma<TY, DV, KT, 64>::N;
+  int j0 = k0 + wave * KT;
+  if (j0 < k1) fetch(j0, mine);
+
+  FwdWave<TY, MAPS, DQ, DV, BIAS> wv;
   wv.init();
   wv.load_q(a, (const T*)a.q + b * a.sq[0] + (ok ? i : 0) * a.sq[1] + h * a.sq[2], ok, half);
   wv.pos = st + (ok ? i : 0);
   wv.pmin = st;
   wv.pmax = st + a.Lq - 1;
-  const int seen = a.causal ? min(nk, max(st + nq, 0)) : nk;
-  wv.limit = ok ? min(seen - 1, a.causal ? wv.pos : seen - 1) : -1;
+  wv.limit = min(k1 - 1, a.causal ? wv.pos : k1 - 1);
+  wv.low = min(k1 - 1, a.causal ? wv.pmin : k1 - 1);
+  wv.c2 = a.scale * LOG2E;
   if constexpr (BIAS) {
     const int n = bias_size(a.reach);
-    for (int t = tid; t < n * G; t += 256) tabs[t] = bias_log2<TY>(a, t % n - a.reach - BIAS_PAD, hk * G + t / n);
+    for (int x = 0; x < G; ++x) fill_bias<TY>(a, tabs + x * n, hk * G + x, tid, 256);
     wv.tab = tabs + (row < R ? g : 0) * n + a.reach + BIAS_PAD;
     wv.far_l = bias_log2<TY>(a, -a.reach, h);
     wv.far_r = bias_log2<TY>(a, a.reach, h);
     wv.fold = !__any(fabsf(wv.far_l) >= BIAS_FOLD || fabsf(wv.far_r) >= BIAS_FOLD);
     __syncthreads();
   }
-  const float c2 = a.scale * LOG2E;
-  const int per = ((seen + splits - 1) / splits + 127) / 128 * 128;      // keys per part: whole rounds of the 4 waves
-  const int k0 = min(sp * per, seen), k1 = min(k0 + per, seen);
-
-  const T* kp = (const T*)a.k + b * a.sk[0] + hk * a.sk[2];
-  const T* vp = (const T*)a.v + b * a.sv[0] + hk * a.sv[2];
-  Stage<TY, DQ, KT, 64> ks[MAPS];
-  Stage<TY, DV, KT, 64> vs;
-  auto fetch = [&](int j0) {
-#pragma unroll
-    for (int p = 0; p < MAPS; ++p) ks[p].load(kp + (MAPS == 2 ? p * a.sk[3] : 0), a.sk[1], j0, k1, a.D, lane);
-    vs.load(vp, a.sv[1], j0, k1, a.Dv, lane);
-  };
-  // each part ends where the next begins: its rows' limit goes no further
-  wv.limit = min(wv.limit, k1 - 1);
-  int j0 = k0 + wave * KT;
-  if (j0 < k1) fetch(j0);
-  for (; j0 < k1; j0 += 4 * KT) {
-#pragma unroll
-    for (int p = 0; p < MAPS; ++p) ks[p].store(mine + p * KT * TK::ROWB, lane);
-    vs.store(mine + KB, lane);
-    if (j0 + 4 * KT < k1) fetch(j0 + 4 * KT);
-    wv.tile(mine, mine + KB, j0, a.reach, c2, lane);
+  for (int buf = 0; j0 < k1; j0 += 4 * KT) {
+    const char* now = mine + buf * (L::KB + L::VB);
+    const int nx = j0 + 4 * KT;
+    if (L::BUFS == 2 && nx < k1) {
+      buf ^= 1;
+      fetch(nx, mine + buf * (L::KB + L::VB));
+      dma_wait<LOADS>();
+    } else {
+      dma_wait<0>();
+    }
+    wv.template step<KT>(now, L::MB, now + L::KB, 0, j0, a.reach, lane);
+    if (L::BUFS == 1 && nx < k1) {
+      __builtin_amdgcn_s_waitcnt(0xc07f);              // this wave's reads of the tile are done
+      fetch(nx, mine);
+    }
   }
 
   // join the 4 waves: their parts in LDS, over the tiles (every wave is past its last read)
@@ -432,58 +443,59 @@ __global__ __launch_bounds__(256) void attn_step_kernel(AttnArgs a, int splits) 
   }
 }
 
-// One wave a row: the parts' weights from their maxima, then the columns.
+// A wave a row: the parts' weights from their maxima (a lane a part, at most 64), then the columns, a quarter of the parts a lane
+// group so that their loads overlap.
 template <int TY, int MAPS, int DV>
-__global__ __launch_bounds__(64) void attn_join_kernel(AttnArgs a, int splits) {
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int splits, int rows) {
   typedef typename El<TY>::T T;
-  constexpr int REC = DV + 4;
+  constexpr int REC = DV + 4, C = DV / 4, S = 64 / C;  // 16-byte columns of a row; lane groups
+  const int at = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (at >= rows) return;
   const int G = a.H / a.Hkv, R = a.Lq * G;
-  const int bh = blockIdx.x / R, jr = blockIdx.x % R, b = bh / a.Hkv, hk = bh % a.Hkv, lane = threadIdx.x;
+  const int bh = at / R, jr = at % R, b = bh / a.Hkv, hk = bh % a.Hkv;
   const int qi = jr / G, qh = hk * G + jr % G;
   if (qi >= clamp_len(a.q_len, b, a.Lq)) return;
-  constexpr int C = DV > 64 ? 2 : 1;                   // columns lane, lane + 64
-  float y[MAPS][C];
+  const int col = 4 * (lane % C), grp = lane / C;
+  f32x4 y[MAPS];
 #pragma unroll
   for (int p = 0; p < MAPS; ++p) {
     const float* base = a.ws + (((long)bh * MAPS + p) * R + jr) * REC;
     const long step = (long)a.B * a.Hkv * MAPS * R * REC;
-    float mm = -INFINITY, lt = 0.0f;
-    for (int s = lane; s < splits; s += 64) mm = fmaxf(mm, base[s * step + DV]);
+    const float m = lane < splits ? base[lane * step + DV] : -INFINITY;
+    const float l = lane < splits ? base[lane * step + DV + 1] : 0.0f;
+    float mm = m;
 #pragma unroll
     for (int d = 32; d; d >>= 1) mm = fmaxf(mm, __shfl_xor(mm, d));
-#pragma unroll
-    for (int c = 0; c < C; ++c) y[p][c] = 0.0f;
-    for (int s = 0; s < splits; ++s) {
-      const float* r = base + s * step;
-      const float wgt = r[DV] == -INFINITY ? 0.0f : exp2_(r[DV] - mm);
-      lt = fmaf(wgt, r[DV + 1], lt);
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-        if (lane + 64 * c < DV) y[p][c] = fmaf(wgt, r[lane + 64 * c], y[p][c]);
+    const float w = m == -INFINITY ? 0.0f : exp2_(m - mm);
+    const float lt = wave_sum(w * l);
+    f32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int s0 = 0; s0 < splits; s0 += S) {
+      const int s = s0 + grp;
+      const float ws = __shfl(w, min(s, 63));
+      if (s < splits) t += ws * *reinterpret_cast<const f32x4*>(base + s * step + col);
     }
-    const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
 #pragma unroll
-    for (int c = 0; c < C; ++c) y[p][c] *= inv;
+    for (int d = C; d < 64; d <<= 1)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) t[r] += __shfl_xor(t[r], d);
+    y[p] = t * (lt == 0.0f ? 0.0f : 1.0f / lt);
     if (a.stats && lane == 0) {
       float* s = a.stats + 2 * ((((long)p * a.B + b) * a.H + qh) * a.Lq + qi);
       s[0] = lt == 0.0f ? 0.0f : mm;
       s[1] = lt == 0.0f ? INFINITY : log2f(lt);
     }
   }
-  float lam = 0.0f;
+  f32x4 x = y[0];
   if constexpr (MAPS == 2) {
     float e1, e2;
-    lam = diff_lambda<TY>(a, e1, e2);
-  }
-  T* op = (T*)a.out + b * a.so[0] + qi * a.so[1] + qh * a.so[2];
-  T* o2 = (MAPS == 2 && a.out2) ? (T*)a.out2 + (((long)b * a.Lq + qi) * a.H + qh) * a.Dv : nullptr;
+    const float lam = diff_lambda<TY>(a, e1, e2);
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int col = lane + 64 * c;
-    if (col >= a.Dv) continue;
-    El<TY>::store(op + col, MAPS == 2 ? fmaf(-lam, y[MAPS - 1][c], y[0][c]) : y[0][c]);
-    if (MAPS == 2 && o2) El<TY>::store(o2 + col, y[MAPS - 1][c]);
+    for (int r = 0; r < 4; ++r) x[r] = fmaf(-lam, y[1][r], x[r]);
   }
+  if (grp || col >= a.Dv) return;
+  El<TY>::store4((T*)a.out + b * a.so[0] + qi * a.so[1] + qh * a.so[2] + col, x);
+  if (MAPS == 2 && a.out2) El<TY>::store4((T*)a.out2 + (((long)b * a.Lq + qi) * a.H + qh) * a.Dv + col, y[MAPS - 1]);
 }
 
 // ---- host ----------------------------------------------------------------------------------------
@@ -499,7 +511,7 @@ static int step_splits(const AttnArgs* a) {
   const long groups = (long)a->B * a->Hkv;
   long s = (1024 + groups - 1) / groups, most = (a->Lk + 255) / 256;
   if (s > most) s = most;
-  return s < 1 ? 1 : (int)s;
+  return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }
 
 template <int TY, int MAPS, int DQ, int DV, bool BIAS>
@@ -510,14 +522,14 @@ static int launch_fwd(const AttnArgs* a, hipStream_t stream) {
     const int splits = step_splits(a), G = a->H / a->Hkv;
     const long rows = (long)a->B * a->Hkv * MAPS * a->Lq * G;
     if (splits > 1 && (!a->ws || a->ws_floats < splits * rows * (DV + 4))) return SGTA_EBADARG;
-    int lds = 4 * 32 * (MAPS * DQ + DV) * SZ + G * tab;
-    const int join = 4 * 32 * (DV + 4) * 4;
-    if (lds < join) lds = join;
+    typedef StepTile<TY, MAPS, DQ, DV> L;
+    const int lds = L::LDS + G * tab > L::JOIN ? L::LDS + G * tab : L::JOIN;
     if (int e = allow_lds<attn_step_kernel<TY, MAPS, DQ, DV, BIAS>>(lds)) return e;
     hipLaunchKernelGGL((attn_step_kernel<TY, MAPS, DQ, DV, BIAS>), dim3(a->B * a->Hkv * splits), dim3(256), lds, stream, *a, splits);
     SGTA_LAUNCH_CHECK();
     if (splits > 1) {
-      hipLaunchKernelGGL((attn_join_kernel<TY, MAPS, DV>), dim3(a->B * a->Hkv * a->Lq * G), dim3(64), 0, stream, *a, splits);
+      const int rows1 = a->B * a->H * a->Lq;
+      hipLaunchKernelGGL((attn_join_kernel<TY, MAPS, DV>), dim3(cdiv(rows1, 4)), dim3(256), 0, stream, *a, splits, rows1);
       SGTA_LAUNCH_CHECK();
     }
     return SGTA_OK;
@@ -542,6 +554,8 @@ int attn_check(const AttnArgs* a, int maps) {
   const int al = a->dtype == TY_F32 ? 4 : 8;           // strides and pointers: whole 16-byte pieces
   const long* s[] = {a->sq, a->sk, a->sv, a->so};
   const void* p[] = {a->q, a->k, a->v, a->out};
+  for (int i = 0; i < 3; ++i)
+    if (s[i][1] > MAX_PITCH / (a->dtype == TY_F32 ? 4 : 2) || s[i][1] < 0) return SGTA_ETOOBIG;
   for (int i = 0; i < 4; ++i) {
     if ((uintptr_t)p[i] % 16) return SGTA_EBADARG;
     for (int j = 0; j < (i < 2 && maps == 2 ? 4 : 3); ++j)

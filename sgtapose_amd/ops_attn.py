@@ -6,7 +6,7 @@
 Element types float32, float16, bfloat16 (one for all tensors of a call); sums, softmax statistics and the bias are held in
 float32.  Query head h reads key / value head h // (H // Hkv).  The last dimension is contiguous; the others may have any
 non-negative stride of whole 16 bytes (slices of a fused projection, caches).  D and Dv are multiples of 8: up to 128 for
-``rel_attention`` (Dv = D), up to 64 and 128 for ``diff_attention``.
+``rel_attention`` (Dv = D), up to 64 and 128 for ``diff_attention``.  Positions lie at most 16 MB apart.
 
 Lengths: ``kv_len`` / ``q_len`` int32 [B] on the GPU (None: all).  What lies behind them is never read, output rows behind
 ``q_len`` are left as they are (an output that a call allocates itself holds zeros there).  ``q_start`` int32 [B] is the position of
@@ -25,6 +25,7 @@ import torch
 from . import _lib
 
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+MAX_PITCH = 1 << 24            # bytes from one position to the next
 MAX_REACH = 1024               # distances that may have buckets of their own (the kernels keep them in LDS)
 
 
@@ -45,6 +46,7 @@ def _first_distances(n, far):
     return out
 
 
+@functools.lru_cache(maxsize=None)
 def bucket_reach(num_buckets, max_distance, bidirectional):
     """The distance from which on the bucket stays the same (checks the arguments)."""
     n = num_buckets // 2 if bidirectional else num_buckets
@@ -71,49 +73,47 @@ def relative_buckets(num_buckets, max_distance, bidirectional):
 
 @functools.lru_cache(maxsize=None)
 def _lut(num_buckets, max_distance, bidirectional, device):
-    """``relative_buckets`` on the device: depends on nothing but the arguments, as ops.gauss_taps."""
-    return torch.tensor(relative_buckets(num_buckets, max_distance, bidirectional), dtype=torch.int32).to(device)
+    """``relative_buckets`` on the device, and each bucket's first entry and number of entries: depends on nothing but the arguments,
+    as ops.gauss_taps."""
+    of = relative_buckets(num_buckets, max_distance, bidirectional)
+    count = [of.count(b) for b in range(num_buckets)]
+    first = [of.index(b) if n else 0 for b, n in enumerate(count)]
+    return torch.tensor(of + first + count, dtype=torch.int32).to(device)
 
 
-def _strides(t, maps):
+def _whole(name, shape, stride, size):
+    """Checks a strided operand's layout -> its strides, those of dimensions of one element (which torch leaves arbitrary) set to
+    what a kernel may multiply."""
+    whole = 16 // size
+    st = [s if n > 1 else whole for s, n in zip(stride[:-1], shape[:-1])]
+    if (stride[-1] != 1 and shape[-1] != 1) or any(s % whole or s < 0 for s in st):
+        _fail("%s: the last dimension must be contiguous, the other strides whole 16 bytes (strides %s)", name, tuple(stride))
+    if st[1] * size > MAX_PITCH:
+        _fail("%s: positions lie at most %d bytes apart (strides %s)", name, MAX_PITCH, tuple(stride))
+    return st
+
+
+def _set_strides(a, field, st, map_dim):
     """Element strides {batch, position, head, map} of [B, L, heads(, 2), D]."""
-    s = t.stride()
-    return (ctypes.c_long * 4)(s[0], s[1], s[2], s[3] if maps == 2 else 0)
+    f = getattr(a, field)
+    f[0], f[1], f[2], f[3] = st[0], st[1], st[2], st[3] if map_dim else 0
 
 
-def _layout(name, t, shape, like):
-    """Shape, type, device and 16-byte layout of one strided operand."""
-    if tuple(t.shape) != tuple(shape):
-        _fail("%s is %s, expected %s", name, tuple(t.shape), tuple(shape))
-    if t.dtype != like.dtype or t.device != like.device:
-        _fail("%s is %s on %s, q is %s on %s", name, t.dtype, t.device, like.dtype, like.device)
-    whole = 16 // t.element_size()
-    if t.stride(-1) != 1 or any(s % whole or s < 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1) or t.data_ptr() % 16:
-        _fail("%s: the last dimension must be contiguous, the others' strides and the pointer whole 16 bytes (strides %s)",
-              name, tuple(t.stride()))
-
-
-def _dense(t):
-    """``t`` with the strides of dimensions of one element set to what a kernel may multiply (torch leaves them arbitrary)."""
-    if any(n == 1 for n in t.shape[:-1]):
-        whole = 16 // t.element_size()
-        t = t.as_strided(t.shape, [s if n > 1 or i == t.dim() - 1 else whole for i, (s, n) in enumerate(zip(t.stride(), t.shape))])
-    return t
-
-
-def _operands(maps, q, k, v, w, causal, scale, q_len, kv_len, q_start):
-    """Checks what every call has in common -> AttnArgs (w and outputs still to be set)."""
-    mp = (2,) if maps == 2 else ()
-    nd = 4 + len(mp)
-    if q.dim() != nd or k.dim() != nd or v.dim() != 4:
-        _fail("q %s, k %s, v %s: expected [B, L, heads%s, D] and [B, L, heads, Dv]", tuple(q.shape), tuple(k.shape), tuple(v.shape),
-              ", 2" if mp else "")
-    if q.dtype not in DTYPES:
-        _fail("attention takes float32, float16 or bfloat16, got %s", q.dtype)
-    B, Lq, H, D = q.shape[0], q.shape[1], q.shape[2], q.shape[-1]
-    Lk, Hkv, Dv = v.shape[1], v.shape[2], v.shape[3]
+@functools.lru_cache(maxsize=1024)
+def _plan(maps, qs, qst, ks, kst, vs, vst, dtype, causal, scale, w_shape, max_distance, bidirectional, lam_init):
+    """Everything that follows from shapes, strides and settings: the checks, and AttnArgs with all but pointers."""
+    nd = 5 if maps == 2 else 4
+    if len(qs) != nd or len(ks) != nd or len(vs) != 4:
+        _fail("q %s, k %s, v %s: expected [B, L, heads%s, D] and [B, L, heads, Dv]", tuple(qs), tuple(ks), tuple(vs), ", 2" if maps == 2 else "")
+    if dtype not in DTYPES:
+        _fail("attention takes float32, float16 or bfloat16, got %s", dtype)
+    B, Lq, H, D = qs[0], qs[1], qs[2], qs[-1]
+    Lk, Hkv, Dv = vs[1], vs[2], vs[3]
     if min(B, Lq, Lk, H, Hkv) < 1 or H % Hkv:
         _fail("B %d, Lq %d, Lk %d, %d heads on %d key / value heads: none may be zero, the heads shared evenly", B, Lq, Lk, H, Hkv)
+    mp = (2,) if maps == 2 else ()
+    if tuple(qs) != (B, Lq, H, *mp, D) or tuple(ks) != (B, Lk, Hkv, *mp, D) or vs[0] != B:
+        _fail("q %s, k %s, v %s do not fit together", tuple(qs), tuple(ks), tuple(vs))
     most = (128, 128) if maps == 1 else (64, 128)
     if D % 8 or Dv % 8 or not 8 <= D <= most[0] or not 8 <= Dv <= most[1] or (maps == 1 and D != Dv):
         _fail("head sizes %d, %d: multiples of 8 up to %d, %d%s", D, Dv, *most, ", equal" if maps == 1 else "")
@@ -123,25 +123,65 @@ def _operands(maps, q, k, v, w, causal, scale, q_len, kv_len, q_start):
         scale = D ** -0.5
     if not (scale > 0 and math.isfinite(scale)):
         _fail("scale %r: a positive number", scale)
-    _layout("q", q, (B, Lq, H, *mp, D), q)
-    _layout("k", k, (B, Lk, Hkv, *mp, D), q)
-    _layout("v", v, (B, Lk, Hkv, Dv), q)
-    for name, t in (("q_len", q_len), ("kv_len", kv_len), ("q_start", q_start)):
-        if t is not None and (tuple(t.shape) != (B,) or t.dtype != torch.int32 or t.device != q.device or not t.is_contiguous()):
-            _fail("%s: int32 [%d] on %s expected, got %s %s on %s", name, B, q.device, t.dtype, tuple(t.shape), t.device)
-    if w.dtype != q.dtype or w.device != q.device or not w.is_contiguous():
-        _fail("the learned weights are %s on %s: %s, contiguous, on %s expected", w.dtype, w.device, q.dtype, q.device)
-    if not q.is_cuda:
-        _fail("expected tensors on the GPU, got %s (there is no CPU fallback)", q.device)
-    q, k, v = _dense(q), _dense(k), _dense(v)
-    a = _lib.AttnArgs(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), w=w.data_ptr(), sq=_strides(q, maps), sk=_strides(k, maps),
-                      sv=_strides(v, 1), B=B, Lq=Lq, Lk=Lk, H=H, Hkv=Hkv, D=D, Dv=Dv, causal=int(causal), dtype=DTYPES[q.dtype],
-                      scale=scale, q_len=_ptr(q_len), kv_len=_ptr(kv_len), q_start=_ptr(q_start))
+    a = _lib.AttnArgs(B=B, Lq=Lq, Lk=Lk, H=H, Hkv=Hkv, D=D, Dv=Dv, causal=int(causal), dtype=DTYPES[dtype], scale=scale)
+    size = 4 if dtype == torch.float32 else 2
+    _set_strides(a, "sq", _whole("q", qs, qst, size), maps == 2)
+    _set_strides(a, "sk", _whole("k", ks, kst, size), maps == 2)
+    _set_strides(a, "sv", _whole("v", vs, vst, size), False)
+    if maps == 1:
+        if len(w_shape) != 2 or w_shape[1] != H:
+            _fail("table is %s, expected [num_buckets, %d]", tuple(w_shape), H)
+        a.num_buckets, a.reach = w_shape[0], bucket_reach(w_shape[0], max_distance, bidirectional)
+    else:
+        if tuple(w_shape) != (4, D):
+            _fail("lam is %s, expected [4, %d]", tuple(w_shape), D)
+        a.lam_init = lam_init
+    a.so[0], a.so[1], a.so[2] = Lq * H * Dv, H * Dv, Dv
     return a
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+def _operands(maps, q, k, v, w, causal, scale, q_len, kv_len, q_start, max_distance=0, bidirectional=False, lam_init=0.0):
+    """Checks what every call has in common -> AttnArgs (outputs still to be set)."""
+    dev, dtype = q.device, q.dtype
+    scale = None if scale is None else float(scale)
+    a = _lib.AttnArgs.from_buffer_copy(_plan(maps, q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), dtype, bool(causal), scale,
+                                             w.shape, max_distance, bidirectional, lam_init))
+    for name, t in (("k", k), ("v", v), ("the learned weights", w)):
+        if t.dtype != dtype or t.device != dev:
+            _fail("%s: %s on %s, q is %s on %s", name, t.dtype, t.device, dtype, dev)
+    if not w.is_contiguous():
+        _fail("the learned weights must be contiguous")
+    a.q, a.k, a.v, a.w = pq, pk, pv, _ = q.data_ptr(), k.data_ptr(), v.data_ptr(), w.data_ptr()
+    if (pq | pk | pv) & 15:
+        _fail("q, k and v must start at whole 16 bytes")
+    if q_len is not None:
+        a.q_len = _lengths("q_len", q_len, a.B, dev)
+    if kv_len is not None:
+        a.kv_len = _lengths("kv_len", kv_len, a.B, dev)
+    if q_start is not None:
+        a.q_start = _lengths("q_start", q_start, a.B, dev)
+    if not q.is_cuda:
+        _fail("expected tensors on the GPU, got %s (there is no CPU fallback)", dev)
+    if maps == 1:
+        a.lut = _lut(a.num_buckets, max_distance, bidirectional, dev).data_ptr()
+    return a
+
+
+def _lengths(name, t, B, dev):
+    if t.shape != (B,) or t.dtype != torch.int32 or t.device != dev or (B > 1 and t.stride(0) != 1):
+        _fail("%s: int32 [%d] on %s expected, got %s %s on %s", name, B, dev, t.dtype, tuple(t.shape), t.device)
+    return t.data_ptr()
+
+
+def _like(name, t, shape, like):
+    """A further operand: shape, type, device, layout -> its strides."""
+    if tuple(t.shape) != tuple(shape):
+        _fail("%s is %s, expected %s", name, tuple(t.shape), tuple(shape))
+    if t.dtype != like.dtype or t.device != like.device:
+        _fail("%s is %s on %s, q is %s on %s", name, t.dtype, t.device, like.dtype, like.device)
+    if t.data_ptr() & 15:
+        _fail("%s must start at whole 16 bytes", name)
+    return _whole(name, t.shape, t.stride(), t.element_size())
 
 
 def _overlaps(t):
@@ -154,22 +194,30 @@ def _overlaps(t):
     return False
 
 
-def _output(name, t, shape, like, partial=False):
-    """The caller's tensor, checked, or a new one (zeros where a call may leave rows as they are)."""
+def _output(a, field, strides, t, shape, like, partial):
+    """The caller's tensor, checked, or a new one (zeros where a call may leave rows as they are), set in ``a``."""
     if t is None:
-        return torch.zeros(shape, dtype=like.dtype, device=like.device) if partial else torch.empty(shape, dtype=like.dtype, device=like.device)
-    _layout(name, t, shape, like)
-    if _overlaps(t):
-        _fail("%s: elements that share memory (strides %s) cannot be written", name, tuple(t.stride()))
+        t = (torch.zeros if partial else torch.empty)(shape, dtype=like.dtype, device=like.device)
+        st = t.stride()
+    else:
+        st = _like(field, t, shape, like)
+        if _overlaps(t):
+            _fail("%s: elements that share memory (strides %s) cannot be written", field, tuple(t.stride()))
+    setattr(a, field, t.data_ptr())
+    _set_strides(a, strides, st, len(shape) == 5)
     return t
 
 
-def _work(floats, device):
-    return torch.empty(floats, dtype=torch.float32, device=device) if floats else None
-
-
-def _enqueue(name, a, device, meta):
-    _lib.call(name, ctypes.byref(a), ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream), meta=meta)
+def _enqueue(name, a, device, ws_name, maps, meta):
+    """Launches on the device's current stream, with the workspace the call needs."""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _enqueue(name, a, device, ws_name, maps, meta)
+    n = getattr(_lib.load(), ws_name)(ctypes.byref(a), maps)
+    if n:
+        ws = torch.empty(n, dtype=torch.float32, device=device)
+        a.ws, a.ws_floats = ws.data_ptr(), n
+    _lib.call(name, ctypes.byref(a), torch.cuda.current_stream(device).cuda_stream, meta=meta)
 
 
 def _meta(kernel, a, maps, products):
@@ -183,22 +231,9 @@ def _meta(kernel, a, maps, products):
             "bytes": size * (a.B * a.Lq * a.H * (maps * a.D + a.Dv) + a.B * a.Lk * a.Hkv * (maps * a.D + a.Dv))}
 
 
-def _check_table(table, H, max_distance, bidirectional):
-    if table.dim() != 2 or table.shape[1] != H:
-        _fail("table is %s, expected [num_buckets, %d]", tuple(table.shape), H)
-    return bucket_reach(table.shape[0], int(max_distance), bool(bidirectional))
-
-
-def _check_lam(lam, D):
-    if tuple(lam.shape) != (4, D):
-        _fail("lam is %s, expected [4, %d]", tuple(lam.shape), D)
-
-
 def _forward(name, maps, a, like, out, q_len, save):
     shape = (a.B, a.Lq, a.H, a.Dv)
-    out = _output("out", out, shape, like, partial=q_len is not None)
-    o = _dense(out)
-    a.out, a.so = o.data_ptr(), _strides(o, 1)
+    out = _output(a, "out", "so", out, shape, like, q_len is not None)
     stats = out2 = None
     if save:
         stats = torch.empty(maps, a.B, a.H, a.Lq, 2, dtype=torch.float32, device=like.device)
@@ -206,10 +241,7 @@ def _forward(name, maps, a, like, out, q_len, save):
         if maps == 2:
             out2 = torch.empty(shape, dtype=like.dtype, device=like.device)
             a.out2 = out2.data_ptr()
-    ws = _work(_lib.load().sgta_attn_fwd_ws_floats(ctypes.byref(a), maps), like.device)
-    if ws is not None:
-        a.ws, a.ws_floats = ws.data_ptr(), ws.numel()
-    _enqueue(name, a, like.device, _meta(name, a, maps, (maps, maps)))
+    _enqueue(name, a, like.device, "sgta_attn_fwd_ws_floats", maps, _meta(name, a, maps, (maps, maps)))
     return (out, (stats, out2)) if save else out
 
 
@@ -219,48 +251,39 @@ def rel_attention(q, k, v, table, out=None, *, max_distance=128, bidirectional=T
 
     ``table`` [num_buckets, H] is the learned bias; buckets as ``relative_buckets(num_buckets, max_distance, bidirectional)``.
     ``scale`` None: D ** -0.5.  ``save``: returns (out, saved) for ``rel_attention_bwd``."""
-    reach = _check_table(table, q.shape[2], max_distance, bidirectional)
-    a = _operands(1, q, k, v, table, causal, scale, q_len, kv_len, q_start)
-    with torch.cuda.device(q.device):
-        lut = _lut(table.shape[0], int(max_distance), bool(bidirectional), q.device)
-        a.lut, a.reach, a.num_buckets = lut.data_ptr(), reach, table.shape[0]
-        return _forward("sgta_rel_attn_fwd", 1, a, q, out, q_len, save)
+    a = _operands(1, q, k, v, table, causal, scale, q_len, kv_len, q_start, int(max_distance), bool(bidirectional))
+    return _forward("sgta_rel_attn_fwd", 1, a, q, out, q_len, save)
 
 
 def diff_attention(q, k, v, lam, out=None, *, lam_init=0.8, causal=False, scale=None, q_len=None, kv_len=None, q_start=None, save=False):
     """(softmax(scale q1 k1^T) - lambda softmax(scale q2 k2^T)) v; ``lam`` [4, D] holds the learned vectors of
     lambda = exp(lam[0].lam[1]) - exp(lam[2].lam[3]) + lam_init, one for all heads.  V is read once for both maps.
     ``save``: returns (out, saved) for ``diff_attention_bwd``."""
-    _check_lam(lam, q.shape[-1])
-    a = _operands(2, q, k, v, lam, causal, scale, q_len, kv_len, q_start)
-    a.lam_init = lam_init
-    with torch.cuda.device(q.device):
-        return _forward("sgta_diff_attn_fwd", 2, a, q, out, q_len, save)
+    a = _operands(2, q, k, v, lam, causal, scale, q_len, kv_len, q_start, lam_init=float(lam_init))
+    return _forward("sgta_diff_attn_fwd", 2, a, q, out, q_len, save)
 
 
 def _backward(name, maps, a, like, dout, w, out, saved, grads, q_len, kv_len):
     mp = (2,) if maps == 2 else ()
     stats, out2 = saved
     shape = (a.B, a.Lq, a.H, a.Dv)
-    _layout("dout", dout, shape, like)
-    _layout("out", out, shape, like)
+    _set_strides(a, "sdo", _like("dout", dout, shape, like), False)
+    _set_strides(a, "so", _like("out", out, shape, like), False)
     if tuple(stats.shape) != (maps, a.B, a.H, a.Lq, 2) or stats.device != like.device or (maps == 2 and tuple(out2.shape) != shape):
         _fail("saved does not come from a forward call of this shape")
+    a.dout, a.out, a.stats = dout.data_ptr(), out.data_ptr(), stats.data_ptr()
+    if maps == 2:
+        a.out2 = out2.data_ptr()
     dq, dk, dv, dw = grads
-    dq = _output("dq", dq, (a.B, a.Lq, a.H, *mp, a.D), like, q_len is not None)
-    dk = _output("dk", dk, (a.B, a.Lk, a.Hkv, *mp, a.D), like, kv_len is not None)
-    dv = _output("dv", dv, (a.B, a.Lk, a.Hkv, a.Dv), like, kv_len is not None)
+    dq = _output(a, "dq", "sdq", dq, (a.B, a.Lq, a.H, *mp, a.D), like, q_len is not None)
+    dk = _output(a, "dk", "sdk", dk, (a.B, a.Lk, a.Hkv, *mp, a.D), like, kv_len is not None)
+    dv = _output(a, "dv", "sdv", dv, (a.B, a.Lk, a.Hkv, a.Dv), like, kv_len is not None)
     if dw is None:
         dw = torch.empty_like(w)
     elif dw.shape != w.shape or dw.dtype != w.dtype or dw.device != w.device or not dw.is_contiguous():
         _fail("the learned weights' gradient is %s %s, expected %s %s, contiguous", dw.dtype, tuple(dw.shape), w.dtype, tuple(w.shape))
-    g, o, q_, k_, v_ = (_dense(t) for t in (dout, out, dq, dk, dv))
-    a.dout, a.sdo, a.out, a.so = g.data_ptr(), _strides(g, 1), o.data_ptr(), _strides(o, 1)
-    a.dq, a.sdq, a.dk, a.sdk, a.dv, a.sdv = q_.data_ptr(), _strides(q_, maps), k_.data_ptr(), _strides(k_, maps), v_.data_ptr(), _strides(v_, 1)
-    a.dw, a.stats, a.out2 = dw.data_ptr(), stats.data_ptr(), _ptr(out2)
-    ws = _work(_lib.load().sgta_attn_bwd_ws_floats(ctypes.byref(a), maps), like.device)
-    a.ws, a.ws_floats = ws.data_ptr(), ws.numel()
-    _enqueue(name, a, like.device, _meta(name, a, maps, (5 * maps, 3)))
+    a.dw = dw.data_ptr()
+    _enqueue(name, a, like.device, "sgta_attn_bwd_ws_floats", maps, _meta(name, a, maps, (5 * maps, 3)))
     return dq, dk, dv, dw
 
 
@@ -269,19 +292,12 @@ def rel_attention_bwd(dout, q, k, v, table, out, saved, dq=None, dk=None, dv=Non
     """Gradients (dq, dk, dv, dtable) of ``rel_attention`` for the gradient ``dout`` of its ``out``; the other arguments as in the
     forward call, ``saved`` from its ``save=True``.  Shared heads' gradients are summed; rows behind q_len / kv_len are left as they
     are (zeros where allocated here).  The same inputs give the same bits."""
-    reach = _check_table(table, q.shape[2], max_distance, bidirectional)
-    a = _operands(1, q, k, v, table, causal, scale, q_len, kv_len, q_start)
-    with torch.cuda.device(q.device):
-        lut = _lut(table.shape[0], int(max_distance), bool(bidirectional), q.device)
-        a.lut, a.reach, a.num_buckets = lut.data_ptr(), reach, table.shape[0]
-        return _backward("sgta_rel_attn_bwd", 1, a, q, dout, table, out, saved, (dq, dk, dv, dtable), q_len, kv_len)
+    a = _operands(1, q, k, v, table, causal, scale, q_len, kv_len, q_start, int(max_distance), bool(bidirectional))
+    return _backward("sgta_rel_attn_bwd", 1, a, q, dout, table, out, saved, (dq, dk, dv, dtable), q_len, kv_len)
 
 
 def diff_attention_bwd(dout, q, k, v, lam, out, saved, dq=None, dk=None, dv=None, dlam=None, *, lam_init=0.8, causal=False, scale=None,
                        q_len=None, kv_len=None, q_start=None):
     """Gradients (dq, dk, dv, dlam) of ``diff_attention``, as ``rel_attention_bwd``; dlam [4, D]."""
-    _check_lam(lam, q.shape[-1])
-    a = _operands(2, q, k, v, lam, causal, scale, q_len, kv_len, q_start)
-    a.lam_init = lam_init
-    with torch.cuda.device(q.device):
-        return _backward("sgta_diff_attn_bwd", 2, a, q, dout, lam, out, saved, (dq, dk, dv, dlam), q_len, kv_len)
+    a = _operands(2, q, k, v, lam, causal, scale, q_len, kv_len, q_start, lam_init=float(lam_init))
+    return _backward("sgta_diff_attn_bwd", 2, a, q, dout, lam, out, saved, (dq, dk, dv, dlam), q_len, kv_len)

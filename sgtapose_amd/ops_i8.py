@@ -7,8 +7,6 @@
 x, bias and out are float32, float16 or bfloat16; scales are float32; the sums are exact whole numbers.  Everything is enqueued on
 the current stream of the tensors' device.
 """
-import ctypes
-
 import torch
 
 from . import _lib
@@ -19,19 +17,20 @@ MAX_K = 131071                 # 127 * 128 * K stays below 2^31
 
 def _rows(name, t, dtypes, shape=None):
     """2-D rows of consecutive elements on the GPU; returns their stride."""
-    if t.dim() != 2 or t.dtype not in dtypes or (shape is not None and tuple(t.shape) != tuple(shape)):
+    if t.dim() != 2 or t.dtype not in dtypes or (shape is not None and t.shape != shape):
         _fail("%s: %s %s where %s of %s is expected", name, t.dtype, tuple(t.shape), "a matrix" if shape is None else list(shape),
               " / ".join(str(d).replace("torch.", "") for d in dtypes))
     M, K = t.shape
     if M < 1 or K < 1:
         _fail("%s is empty: %s", name, tuple(t.shape))
-    if (K > 1 and t.stride(1) != 1) or (M > 1 and t.stride(0) < K):
+    ld, one = t.stride()
+    if (K > 1 and one != 1) or (M > 1 and ld < K):
         _fail("%s: rows of consecutive elements that do not overlap expected, strides %s", name, tuple(t.stride()))
-    return t.stride(0) if M > 1 else max(K, t.stride(0))
+    return ld if M > 1 else max(K, ld)
 
 
 def _vector(name, t, n, dtype):
-    if tuple(t.shape) != (n,) or t.dtype != dtype or (n > 1 and t.stride(0) != 1):
+    if t.shape != (n,) or t.dtype != dtype or (n > 1 and t.stride(0) != 1):
         _fail("%s: %s %s where %s [%d] is expected", name, t.dtype, tuple(t.shape), dtype, n)
 
 
@@ -43,8 +42,11 @@ def _together(first, *others):
         _fail("expected tensors on the GPU, got %s (there is no CPU fallback)", first.device)
 
 
-def _stream(device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+def _enqueue(device, name, *args, meta=None):
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _enqueue(device, name, *args, meta=meta)
+    _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream, meta=meta)
 
 
 def quantize_rows(x, xq=None, xs=None):
@@ -64,9 +66,8 @@ def quantize_rows(x, xq=None, xs=None):
     meta = None
     if _lib.PROFILE is not None:
         meta = {"kernel": "quant_rows_kernel", "flops": 2.0 * M * K, "exec_flops": 2.0 * M * K, "bytes": M * K * (x.element_size() + 1.0)}
-    with torch.cuda.device(x.device):
-        _lib.call("sgta_quant_rows_i8", x.data_ptr(), ldx, DTYPES[x.dtype], xq.data_ptr(), xq.stride(0) if M > 1 else max(K, xq.stride(0)),
-                  xs.data_ptr(), M, K, _stream(x.device), meta=meta)
+    _enqueue(x.device, "sgta_quant_rows_i8", x.data_ptr(), ldx, DTYPES[x.dtype], xq.data_ptr(),
+             xq.stride(0) if M > 1 else max(K, xq.stride(0)), xs.data_ptr(), M, K, meta=meta)
     return xq, xs
 
 
@@ -96,8 +97,7 @@ def linear_i8(xq, xs, wq, ws, bias=None, out=None, relu=False, dtype=None):
     if _lib.PROFILE is not None:
         meta = {"kernel": "linear_i8_kernel", "flops": 2.0 * M * N * K, "exec_flops": 2.0 * M * N * K,
                 "bytes": 1.0 * M * K + N * K + out.element_size() * M * N}
-    with torch.cuda.device(xq.device):
-        _lib.call("sgta_linear_i8", xq.data_ptr(), ldx, xs.data_ptr(), wq.data_ptr(), ldw, ws.data_ptr(),
-                  None if bias is None else bias.data_ptr(), out.data_ptr(), out.stride(0) if M > 1 else max(N, out.stride(0)), M, N, K,
-                  int(relu), DTYPES[dtype], _stream(xq.device), meta=meta)
+    _enqueue(xq.device, "sgta_linear_i8", xq.data_ptr(), ldx, xs.data_ptr(), wq.data_ptr(), ldw, ws.data_ptr(),
+             None if bias is None else bias.data_ptr(), out.data_ptr(), out.stride(0) if M > 1 else max(N, out.stride(0)), M, N, K,
+             int(relu), DTYPES[dtype], meta=meta)
     return out
