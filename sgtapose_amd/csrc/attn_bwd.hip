@@ -16,6 +16,8 @@
 // by a power of two that brings the largest |dO| of the row (dQ) or of all queries of the shared heads (dK) next to one.
 #include "attn_common.h"
 
+#define DIAG 768               // floats of a wave's 16 x 32 tile in rows of 47, with 15 zeros in front
+
 int attn_check(const AttnArgs* a, int maps);
 
 __device__ __forceinline__ float pow2_to_one(float top) {          // 2^-exponent(top), 1 for zero and for what is not finite
@@ -48,10 +50,9 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
   typedef Tile<TY, DQ> TK;
   typedef Tile<TY, DV> TV;
   constexpr int MB = KT * TK::ROWB, KB = MAPS * MB, VB = KT * TV::ROWB;
-  extern __shared__ __align__(16) char smem[];       // 2 x (K maps, V) | bias table | 4 waves x 2 lane halves of sums by distance
+  extern __shared__ __align__(16) char smem[];       // 2 x (K maps, V) | bias table | 4 waves: sums by distance | 4 waves: DIAG
   const BwdWork wk(a, MAPS);
   float* tab = reinterpret_cast<float*>(smem + 2 * (KB + VB));
-  float* hist = tab + wk.nrel;
   __shared__ float red[4];
   const int nblk = wk.nblk, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, half = lane >> 5;
   const int bh = blockIdx.x % (a.B * a.H), b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
@@ -161,15 +162,16 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
   float far_l = 0.0f, far_r = 0.0f, sum_l = 0.0f, sum_r = 0.0f, sum_n = 0.0f, p_l = 0.0f, p_r = 0.0f;
   bool fold = true;
   const float* tb = tab;
-  float* mine = hist;
+  float *hist = nullptr, *diag = nullptr;
   if constexpr (BIAS) {
     fill_bias<TY>(a, tab, h, tid, 256);
-    for (int i = tid; i < 8 * wk.nrel; i += 256) hist[i] = 0.0f;
+    for (int i = tid; i < 4 * (wk.nrel + DIAG); i += 256) tab[wk.nrel + i] = 0.0f;
     far_l = bias_log2<TY>(a, -a.reach, h);
     far_r = bias_log2<TY>(a, a.reach, h);
     fold = fabsf(far_l) < BIAS_FOLD && fabsf(far_r) < BIAS_FOLD;
     tb = tab + a.reach + BIAS_PAD;
-    mine = hist + (2 * wave + half) * wk.nrel + a.reach + BIAS_PAD;
+    hist = tab + (1 + wave) * wk.nrel + a.reach + BIAS_PAD;         // at distance 0
+    diag = tab + 5 * wk.nrel + wave * DIAG + 15;
   }
   const float c2 = a.scale * LOG2E;
   const int wave_last = row0 >= nq ? -1 : a.causal ? min(seen - 1, st + min(row0 + 31, nq - 1)) : seen - 1;
@@ -238,10 +240,23 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
           else if (right) sum_r += all;
           else {
             sum_n += all;
-            // one distance a lane and instruction, the lane halves apart: no two lanes add to one place
-            float* hp = mine + (j0 + 4 * half - pos);
+            // Sums by distance, 16 keys at a time: the tile as rows of 32 with 15 zeros between them (row k at 47 k, the zeros stay),
+            // where the entries of one distance, k - q, lie 48 apart; lane u < 47 adds up those of distance 15 - u.  (LDS atomics
+            // into the sums take two cycles a lane: 16 of them cost 1950 cycles a tile.)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) __hip_atomic_fetch_add(hp + 8 * (r >> 2) + (r & 3), s[r] * irs, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+            for (int hf = 0; hf < 2; ++hf) {
+              asm volatile("" ::: "memory");           // a wave's LDS operations are done in order; the compiler keeps it
+#pragma unroll
+              for (int r = 0; r < 8; ++r) diag[(8 * (r >> 2) + 4 * half + (r & 3)) * 47 + li] = s[8 * hf + r] * irs;
+              asm volatile("" ::: "memory");
+              float v = 0.0f, w = 0.0f;
+#pragma unroll
+              for (int k = 0; k < 16; k += 2) {
+                v += diag[48 * k + min(lane, 46) - 15];
+                w += diag[48 * (k + 1) + min(lane, 46) - 15];
+              }
+              if (lane < 47) hist[j0 + 16 * hf - pmin + 15 - lane] += v + w;
+            }
           }
         }
 #pragma unroll
@@ -284,15 +299,13 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
     sum_l = wave_sum(ok ? fmaf(-e, p_l, sum_l) : 0.0f);
     sum_r = wave_sum(ok ? fmaf(-e, p_r, sum_r) : 0.0f);
     if (lane == 0) {                                  // the ends of the table stand for everything beyond
-      hist[2 * wave * wk.nrel] += sum_l;
-      hist[2 * wave * wk.nrel + wk.nrel - 1] += sum_r;
+      tab[(1 + wave) * wk.nrel] += sum_l;
+      tab[(2 + wave) * wk.nrel - 1] += sum_r;
     }
     __syncthreads();
     for (int i = tid; i < wk.nrel; i += 256) {
-      float v = 0.0f;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) v += hist[c * wk.nrel + i];
-      tab[i] = v;                                     // the bias itself is no longer needed
+      // over the bias itself, which is no longer needed
+      tab[i] = (tab[wk.nrel + i] + tab[2 * wk.nrel + i]) + (tab[3 * wk.nrel + i] + tab[4 * wk.nrel + i]);
     }
     __syncthreads();
     // by bucket: a run of distances each, first and count behind the table of buckets; the outermost reach to the table's ends
@@ -428,7 +441,7 @@ __global__ __launch_bounds__(256, (MAPS * DQ + DV > 128 || (TY == TY_F32 && MAPS
       rn = q_first;
     }
     if (it + 1 < steps) fetch(hn, rn, (it & 1) ^ 1);
-#pragma unroll
+#pragma unroll 1
     for (int u = 0; u < QT / 32; ++u) {
       const int q0 = r0 + 32 * u;
       if (q0 + 31 < wave_first || q0 >= nq) continue;
@@ -462,16 +475,19 @@ __global__ __launch_bounds__(256, (MAPS * DQ + DV > 128 || (TY == TY_F32 && MAPS
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[r] = exp2_(BIAS ? fmaf(s[r], c2, far) : s[r] * c2);
         } else {
-          const f32x16 mm = rows16(p, 2), ll = rows16(p, 3);
           const int first = diag ? key - st - q0 - 4 * half : -64;   // register rows from here on see this lane's key
           const float* tp = tab + a.reach + BIAS_PAD + (key - st - q0 - 4 * half);
           const bool near = BIAS && !left && !right;
           const float far = left ? far_l : far_r;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int c = 8 * (r >> 2) + (r & 3);
-            const float e = (fmaf(s[r], c2, !BIAS ? 0.0f : near ? tp[-c] : far) - mm[r]) - ll[r];
-            s[r] = c >= first ? exp2_(e) : 0.0f;
+          for (int c = 0; c < 4; ++c) {
+            const float* sp = stat + 4 * p * QT + 32 * u + 8 * c + 4 * half;
+            const f32x4 mm = *reinterpret_cast<const f32x4*>(sp + 2 * QT), ll = *reinterpret_cast<const f32x4*>(sp + 3 * QT);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float e = (fmaf(s[4 * c + r], c2, !BIAS ? 0.0f : near ? tp[-(8 * c + r)] : far) - mm[r]) - ll[r];
+              s[4 * c + r] = 8 * c + r >= first ? exp2_(e) : 0.0f;
+            }
           }
         }
         if (MAPS == 2 && p == 1) {
@@ -589,7 +605,7 @@ template <int TY, int MAPS, int DQ, int DV, bool BIAS> static int launch_bwd(con
   const BwdWork wk(*a, MAPS);
   const int tab = BIAS ? wk.nrel * 4 : 0;
   constexpr int KT = TY == TY_F32 ? 32 : 64;
-  int lds = 2 * KT * (MAPS * DQ + DV) * SZ + 9 * tab;
+  int lds = 2 * KT * (MAPS * DQ + DV) * SZ + 5 * tab + (BIAS ? 4 * DIAG * 4 : 0);
   if (int e = allow_lds<attn_dq_kernel<TY, MAPS, DQ, DV, BIAS>>(lds)) return e;
   hipLaunchKernelGGL((attn_dq_kernel<TY, MAPS, DQ, DV, BIAS>), dim3(a->B * a->H * wk.nblk), dim3(256), lds, stream, *a);
   SGTA_LAUNCH_CHECK();

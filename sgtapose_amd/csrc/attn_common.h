@@ -75,8 +75,9 @@ __device__ __forceinline__ float wave_sum(float x) {
   return x;
 }
 
-// One operand tile in LDS: rows of COLS elements in 16-byte pieces, XOR-swizzled by the row so that the 8 rows which one
-// quarter of a wave reads at a time fall on different banks.
+// One operand tile in LDS: rows of COLS elements in 16-byte pieces, XOR-swizzled by the row so that what LDS serves at a time
+// falls on different banks: one piece of 8 consecutive rows (read_rows), and two neighbouring pieces of 4 (read_cols; a swizzle
+// by the row number itself puts rows r and r ^ 1 on one pair of pieces: half of these reads' cycles were conflicts).
 template <int TY, int COLS> struct Tile {
   typedef typename El<TY>::T T;
   typedef typename El<TY>::Frag Frag;
@@ -84,7 +85,9 @@ template <int TY, int COLS> struct Tile {
   static constexpr int ROWB = COLS * SZ;              // bytes per row: 64 ... 512
   static constexpr int CH = ROWB / 16;                // pieces per row
   static constexpr int EPC = 16 / SZ;                 // elements per piece
-  static __device__ __forceinline__ int swz(int row) { return ROWB >= 128 ? (row & 7) : ((row >> 1) & 3); }
+  static __device__ __forceinline__ int swz(int row) {
+    return ROWB >= 128 ? ((row & 3) << 1) | ((row >> 2) & 1) : (row & 2) | ((row >> 2) & 1);
+  }
   static __device__ __forceinline__ int piece(int row, int ch) { return row * ROWB + ((ch ^ swz(row)) << 4); }
 
   // operand fragment of row ``row``: elements 16 s + 8 half + 0..7
@@ -202,7 +205,7 @@ __device__ __forceinline__ int start_of(const int* start, int b) { return start 
 // The bias of head h over distances, in LDS: entry [rel + reach + BIAS_PAD] for |rel| <= reach + BIAS_PAD, in units of log2;
 // from ``reach`` on the bucket stays the same.  A tile that comes within ``reach`` of its queries' positions indexes it
 // without a clamp: its distances go at most BIAS_PAD further.
-#define BIAS_PAD 128
+#define BIAS_PAD 96
 __device__ __forceinline__ int bias_size(int reach) { return 2 * (reach + BIAS_PAD) + 1; }
 template <int TY> __device__ __forceinline__ float bias_log2(const AttnArgs& a, int rel, int h) {
   const int at = min(max(rel, -a.reach), a.reach) + a.reach;

@@ -24,6 +24,7 @@ import torch
 
 from . import _lib
 
+raw_stream = torch._C._cuda_getCurrentRawStream      # (device index) -> the current stream's handle; 2 us less a call than the Stream object
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 MAX_PITCH = 1 << 24            # bytes from one position to the next
 MAX_REACH = 1024               # distances that may have buckets of their own (the kernels keep them in LDS)
@@ -217,7 +218,7 @@ def _enqueue(name, a, device, ws_name, maps, meta):
     if n:
         ws = torch.empty(n, dtype=torch.float32, device=device)
         a.ws, a.ws_floats = ws.data_ptr(), n
-    _lib.call(name, ctypes.byref(a), torch.cuda.current_stream(device).cuda_stream, meta=meta)
+    _lib.call(name, ctypes.byref(a), raw_stream(device.index), meta=meta)
 
 
 def _meta(kernel, a, maps, products):
