@@ -110,17 +110,17 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
     for (int s = 0; s < DV / 16; ++s) {
       const int d = 16 * s + 8 * half;
       const bool in = ok && d < a.Dv;
-      g[s] = global_frag<TY>(gp + d, in);
-      const Frag o = global_frag<TY>(op + d, in);
+      const typename El<TY>::Raw gr = global_raw<TY>(gp + d, in), o = global_raw<TY>(op + d, in);
+      g[s] = El<TY>::frag_of(gr);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        s1 = fmaf((float)g[s][e], (float)o[e], s1);
-        top = fmaxf(top, fabsf((float)g[s][e]));
+        s1 = fmaf((float)gr[e], (float)o[e], s1);
+        top = fmaxf(top, fabsf((float)gr[e]));
       }
       if constexpr (MAPS == 2) {
-        const Frag y = global_frag<TY>(o2 + d, in);
+        const typename El<TY>::Raw y = global_raw<TY>(o2 + d, in);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s2 = fmaf((float)g[s][e], (float)y[e], s2);
+        for (int e = 0; e < 8; ++e) s2 = fmaf((float)gr[e], (float)y[e], s2);
       }
     }
     s1 = half_sum(s1);
@@ -174,6 +174,7 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
     diag = tab + 5 * wk.nrel + wave * DIAG + 15;
   }
   const float c2 = a.scale * LOG2E;
+  const bool both = a.D > 16;                         // DQ = 32: the second 16 of the head's elements are not all padding
   const int wave_last = row0 >= nq ? -1 : a.causal ? min(seen - 1, st + min(row0 + 31, nq - 1)) : seen - 1;
 
   f32x16 dq[MAPS][DQ / 32];
@@ -197,13 +198,15 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
       const bool plain = !masked && (!BIAS || (fold && (left || right)));
       f32x16 x = zero16();
 #pragma unroll
-      for (int k = 0; k < DV / 16; ++k) x = El<TY>::mma(TV::read_rows(vt, 32 * u + li, k, half), g[k], x);
+      for (int k = 0; k < DV / 16; ++k)
+        if (DV > 32 || k == 0 || both) x = El<TY>::mma(TV::read_rows(vt, 32 * u + li, k, half), g[k], x);
       Frag df[MAPS][2];
 #pragma unroll
       for (int p = 0; p < MAPS; ++p) {
         f32x16 s = zero16();
 #pragma unroll
-        for (int k = 0; k < DQ / 16; ++k) s = El<TY>::mma(TK::read_rows(kt + p * MB, 32 * u + li, k, half), q[p][k], s);
+        for (int k = 0; k < DQ / 16; ++k)
+          if (DQ > 32 || k == 0 || both) s = El<TY>::mma(TK::read_rows(kt + p * MB, 32 * u + li, k, half), q[p][k], s);
         if (plain) {
           const float add = ((BIAS ? (left ? far_l : far_r) : 0.0f) - m[p]) - lg[p];
 #pragma unroll
@@ -343,6 +346,7 @@ __global__ __launch_bounds__(256, (MAPS * DQ + DV > 128 || (TY == TY_F32 && MAPS
   const int key0 = blk0 + wave * 32, key = key0 + li;
   const bool ok = key < nk;
   const float c2 = a.scale * LOG2E, ic2 = 1.0f / c2;
+  const bool both = a.D > 16;                         // DQ = 32: the second 16 of the head's elements are not all padding
   // under a causal mask the first query that sees key blk0 stands at its position
   const int q_first = a.causal ? min(max(blk0 - st, 0), nq) / QT * QT : 0;
   const int nt = nq > q_first ? (nq - q_first + QT - 1) / QT : 0;
@@ -461,7 +465,8 @@ __global__ __launch_bounds__(256, (MAPS * DQ + DV > 128 || (TY == TY_F32 && MAPS
       };
       f32x16 x = rows16(0, 1);                                       // X - delta: the product starts from -delta
 #pragma unroll
-      for (int k = 0; k < DV / 16; ++k) x = El<TY>::mma(TG::read_rows(gt, 32 * u + li, k, half), vf[k], x);
+      for (int k = 0; k < DV / 16; ++k)
+        if (DV > 32 || k == 0 || both) x = El<TY>::mma(TG::read_rows(gt, 32 * u + li, k, half), vf[k], x);
       f32x16 w0;
       Frag dsf[MAPS][2];
 #pragma unroll
@@ -469,7 +474,8 @@ __global__ __launch_bounds__(256, (MAPS * DQ + DV > 128 || (TY == TY_F32 && MAPS
         f32x16 s = zero16();
         if (plain) s = rows16(p, 0);                                 // and the exponent from (-m - lg) / c2
 #pragma unroll
-        for (int k = 0; k < DQ / 16; ++k) s = El<TY>::mma(TQ::read_rows(qt + p * MB, 32 * u + li, k, half), kf[p][k], s);
+        for (int k = 0; k < DQ / 16; ++k)
+          if (DQ > 32 || k == 0 || both) s = El<TY>::mma(TQ::read_rows(qt + p * MB, 32 * u + li, k, half), kf[p][k], s);
         if (plain) {
           const float far = !BIAS ? 0.0f : left ? far_l : far_r;
 #pragma unroll

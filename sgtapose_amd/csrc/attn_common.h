@@ -1,8 +1,7 @@
 // What the attention kernels share (attn_fwd.hip, attn_bwd.hip): element types, LDS tiles and their fragments, staging.
 //
-// Every product runs on 32x32 matrix tiles: v_mfma_f32_32x32x16_{f16,bf16}, or eight v_mfma_f32_32x32x2_f32 for float, whose
-// operands hold the same (row, 8 k) fragment per lane: lane l has row l & 31 and k = 8 (l >> 5) + 0..7 of a step of 16 (for
-// float, instruction e multiplies element e of both halves: any pairing of k is right as long as both operands use it).
+// Every product runs on 32x32 matrix tiles, v_mfma_f32_32x32x16_{f16,bf16}, float as three bfloat16 numbers.  A lane's operand
+// fragment: lane l has row l & 31 and k = 8 (l >> 5) + 0..7 of a step of 16.
 // A result has its column on the lane (l & 31) and row 8 (r >> 2) + 4 (l >> 5) + (r & 3) in register r.  Eight consecutive
 // result registers are therefore an operand fragment of 16 rows in the order {0-3, 8-11} / {4-7, 12-15} of the two lane
 // halves; read_cols() hands out the other operand in that same order, so softmax weights go from one product into the next
@@ -23,15 +22,53 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 enum { TY_F32 = 0, TY_F16 = 1, TY_BF16 = 2 };
 
 template <int TY> struct El;
+
+// float on the bfloat16 pipe.  A float's 24 significant bits are three bfloat16 numbers, x = hi + mid + lo exactly (each the upper
+// half of what the ones before leave); of the nine products of two such sums the six of at least 2^-16 of the whole are taken, smallest
+// first, each with all its bits into the f32 accumulator: what is left out is below 3 * 2^-24 of |a||b|, the rounding of a few terms.
+// Six v_mfma_f32_32x32x16_bf16 (192 cycles) in place of eight v_mfma_f32_32x32x2_f32 (512), and the splits, ~44 vector
+// instructions a fragment, overlap them.  Same range as float; what is not finite gives not-a-number in hi - hi: so does x * 0.
+struct Split8 {
+  typedef __bf16 x8 __attribute__((ext_vector_type(8)));
+  x8 hi, mid, lo;
+};
+__device__ __forceinline__ unsigned upper_halves(float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); }
+__device__ __forceinline__ Split8 split8(f32x8 v) {
+  typedef unsigned u32x4_ __attribute__((ext_vector_type(4)));
+  u32x4_ h, m, l;
+  f32x8 r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = v[e] - __uint_as_float(__float_as_uint(v[e]) & 0xffff0000u);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    h[e] = upper_halves(v[2 * e], v[2 * e + 1]);
+    m[e] = upper_halves(r[2 * e], r[2 * e + 1]);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] -= __uint_as_float(__float_as_uint(r[e]) & 0xffff0000u);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) l[e] = upper_halves(r[2 * e], r[2 * e + 1]);
+  Split8 s;
+  s.hi = __builtin_bit_cast(Split8::x8, h);
+  s.mid = __builtin_bit_cast(Split8::x8, m);
+  s.lo = __builtin_bit_cast(Split8::x8, l);
+  return s;
+}
+
 template <> struct El<TY_F32> {
   typedef float T;
-  typedef f32x8 Frag;
+  typedef Split8 Frag;         // an operand fragment
+  typedef f32x8 Raw;           // eight elements as they lie in memory
   static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
-    return c;
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.lo, b.hi, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.hi, b.lo, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.mid, b.mid, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.mid, b.hi, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.hi, b.mid, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.hi, b.hi, c, 0, 0, 0);
   }
-  static __device__ __forceinline__ Frag frag(f32x8 v) { return v; }
+  static __device__ __forceinline__ Frag frag(f32x8 v) { return split8(v); }
+  static __device__ __forceinline__ Frag frag_of(Raw v) { return split8(v); }
   static __device__ __forceinline__ float load(const T* p) { return *p; }
   static __device__ __forceinline__ void store4(T* p, f32x4 v) { *reinterpret_cast<f32x4*>(p) = v; }
   static __device__ __forceinline__ void store(T* p, float v) { *p = v; }
@@ -40,7 +77,9 @@ template <bool F16> struct El16 {
   typedef typename H16<F16>::T T;
   typedef typename H16<F16>::x4 x4;
   typedef typename H16<F16>::x8 Frag;
+  typedef Frag Raw;
   static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) { return H16<F16>::mfma32(a, b, c); }
+  static __device__ __forceinline__ Frag frag_of(Raw v) { return v; }
   // to the nearest, without the clamp of the 16-bit feature maps: here what exceeds the half range becomes an infinity, by which
   // a training loop sees that its loss is scaled too far
   static __device__ __forceinline__ Frag frag(f32x8 v) { return __builtin_convertvector(v, Frag); }
@@ -95,7 +134,7 @@ template <int TY, int COLS> struct Tile {
     if constexpr (TY == TY_F32) {
       const f32x4 a = *reinterpret_cast<const f32x4*>(lds + piece(row, 4 * s + 2 * half));
       const f32x4 b = *reinterpret_cast<const f32x4*>(lds + piece(row, 4 * s + 2 * half + 1));
-      return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+      return split8(__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
       return *reinterpret_cast<const Frag*>(lds + piece(row, 2 * s + half));
     }
@@ -104,13 +143,13 @@ template <int TY, int COLS> struct Tile {
   static __device__ __forceinline__ Frag read_cols(const char* lds, int row0, int blk, int lane) {
     if constexpr (TY == TY_F32) {
       const int col = 32 * blk + (lane & 31), half = lane >> 5;
-      Frag f;
+      f32x8 f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int row = row0 + 4 * half + (e & 3) + 8 * (e >> 2);
         f[e] = *reinterpret_cast<const float*>(lds + piece(row, col >> 2) + (col & 3) * 4);
       }
-      return f;
+      return split8(f);
     } else {
       // transposing read: each 16 lanes fetch 4 rows x 16 columns, lane i of them gets column i of the 4 rows
       const int g = lane >> 4, i = lane & 15;
@@ -175,12 +214,15 @@ __device__ __forceinline__ f32x16 zero16() {
 }
 
 // eight consecutive elements of a global row as an operand fragment (zero where ``ok`` is false)
-template <int TY> __device__ __forceinline__ typename El<TY>::Frag global_frag(const typename El<TY>::T* p, bool ok) {
-  typename El<TY>::Frag f;
+template <int TY> __device__ __forceinline__ typename El<TY>::Raw global_raw(const typename El<TY>::T* p, bool ok) {
+  typename El<TY>::Raw f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) f[e] = 0;
-  if (ok) f = *reinterpret_cast<const typename El<TY>::Frag*>(p);
+  if (ok) f = *reinterpret_cast<const typename El<TY>::Raw*>(p);
   return f;
+}
+template <int TY> __device__ __forceinline__ typename El<TY>::Frag global_frag(const typename El<TY>::T* p, bool ok) {
+  return El<TY>::frag_of(global_raw<TY>(p, ok));
 }
 
 // lambda = exp(w0 . w1) - exp(w2 . w3) + init, by one wave; e1, e2: the two exponentials
@@ -206,7 +248,7 @@ __device__ __forceinline__ int start_of(const int* start, int b) { return start 
 // from ``reach`` on the bucket stays the same.  A tile that comes within ``reach`` of its queries' positions indexes it
 // without a clamp: its distances go at most BIAS_PAD further.
 #define BIAS_PAD 96
-__device__ __forceinline__ int bias_size(int reach) { return 2 * (reach + BIAS_PAD) + 1; }
+__host__ __device__ __forceinline__ int bias_size(int reach) { return 2 * (reach + BIAS_PAD) + 1; }
 template <int TY> __device__ __forceinline__ float bias_log2(const AttnArgs& a, int rel, int h) {
   const int at = min(max(rel, -a.reach), a.reach) + a.reach;
   const float t = El<TY>::load((const typename El<TY>::T*)a.w + (long)a.lut[at] * a.H + h);

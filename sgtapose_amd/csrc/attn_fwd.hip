@@ -27,6 +27,7 @@ template <int TY, int MAPS, int DQ, int DV, bool BIAS> struct FwdWave {
   float far_l, far_r;          // its values left and right of ``reach``
   bool fold;                   // both may be folded into the exponent
   float c2;                    // scale in log2 units
+  bool both;                   // DQ = 32: the second 16 of the head's elements are not all padding
 
   __device__ __forceinline__ void init() {
 #pragma unroll
@@ -91,7 +92,8 @@ template <int TY, int MAPS, int DQ, int DV, bool BIAS> struct FwdWave {
       for (int u = 0; u < NS; ++u) {
         s[u] = zero16();
 #pragma unroll
-        for (int k = 0; k < DQ / 16; ++k) s[u] = El<TY>::mma(TK::read_rows(kt + p * mapb, k0 + 32 * u + li, k, half), q[p][k], s[u]);
+        for (int k = 0; k < DQ / 16; ++k)
+          if (DQ > 32 || k == 0 || both) s[u] = El<TY>::mma(TK::read_rows(kt + p * mapb, k0 + 32 * u + li, k, half), q[p][k], s[u]);
       }
       float al;
       bool grown;
@@ -207,6 +209,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a, int nblk) 
   wv.limit = min(nk - 1, a.causal ? wv.pos : nk - 1);                // rows behind the last query: computed, not stored
   wv.low = min(nk - 1, a.causal ? wv.pmin : nk - 1);
   wv.c2 = a.scale * LOG2E;
+  wv.both = a.D > 16;
   if constexpr (BIAS) {
     fill_bias<TY>(a, tab, h, tid, 256);
     wv.tab = tab + a.reach + BIAS_PAD;
@@ -322,9 +325,12 @@ __global__ __launch_bounds__(256) void attn_step_kernel(AttnArgs a, int splits) 
   wv.limit = min(k1 - 1, a.causal ? wv.pos : k1 - 1);
   wv.low = min(k1 - 1, a.causal ? wv.pmin : k1 - 1);
   wv.c2 = a.scale * LOG2E;
+  wv.both = a.D > 16;
   if constexpr (BIAS) {
+    // the tables are read by tiles within ``reach`` of the queries only: most parts of a long cache have none
     const int n = bias_size(a.reach);
-    for (int x = 0; x < G; ++x) fill_bias<TY>(a, tabs + x * n, hk * G + x, tid, 256);
+    if (k1 - 1 - wv.pmin > -a.reach && k0 - wv.pmax < a.reach)
+      for (int x = 0; x < G; ++x) fill_bias<TY>(a, tabs + x * n, hk * G + x, tid, 256);
     wv.tab = tabs + (row < R ? g : 0) * n + a.reach + BIAS_PAD;
     wv.far_l = bias_log2<TY>(a, -a.reach, h);
     wv.far_r = bias_log2<TY>(a, a.reach, h);
@@ -350,7 +356,7 @@ __global__ __launch_bounds__(256) void attn_step_kernel(AttnArgs a, int splits) 
 
   // join the 4 waves: their parts in LDS, over the tiles (every wave is past its last read)
   float lam = 0.0f;
-  if constexpr (MAPS == 2) {
+  if (MAPS == 2 && splits == 1) {
     float e1, e2;
     lam = diff_lambda<TY>(a, e1, e2);
   }
@@ -443,8 +449,8 @@ __global__ __launch_bounds__(256) void attn_step_kernel(AttnArgs a, int splits) 
   }
 }
 
-// A wave a row: the parts' weights from their maxima (a lane a part, at most 64), then the columns, a quarter of the parts a lane
-// group so that their loads overlap.
+// A wave a row: the parts' weights from their maxima (a lane a part, at most 64), then the columns, 16 bytes a lane, the lane groups
+// sharing the parts.
 template <int TY, int MAPS, int DV>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int splits, int rows) {
   typedef typename El<TY>::T T;
@@ -455,25 +461,42 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int splits, 
   const int bh = at / R, jr = at % R, b = bh / a.Hkv, hk = bh % a.Hkv;
   const int qi = jr / G, qh = hk * G + jr % G;
   if (qi >= clamp_len(a.q_len, b, a.Lq)) return;
+  float lam = 0.0f;
+  if constexpr (MAPS == 2) {
+    float e1, e2;
+    lam = diff_lambda<TY>(a, e1, e2);
+  }
   const int col = 4 * (lane % C), grp = lane / C;
-  f32x4 y[MAPS];
+  const float* base = a.ws + ((long)bh * MAPS * R + jr) * REC;
+  const long step = (long)a.B * a.Hkv * MAPS * R * REC, map = (long)R * REC;
+  constexpr int AHEAD = 8;                             // parts a lane fetches before it knows their weights
+  f32x4 y[MAPS], first[MAPS][AHEAD];
+  float m[MAPS], l[MAPS];
 #pragma unroll
   for (int p = 0; p < MAPS; ++p) {
-    const float* base = a.ws + (((long)bh * MAPS + p) * R + jr) * REC;
-    const long step = (long)a.B * a.Hkv * MAPS * R * REC;
-    const float m = lane < splits ? base[lane * step + DV] : -INFINITY;
-    const float l = lane < splits ? base[lane * step + DV + 1] : 0.0f;
-    float mm = m;
+    m[p] = lane < splits ? base[p * map + lane * step + DV] : -INFINITY;
+    l[p] = lane < splits ? base[p * map + lane * step + DV + 1] : 0.0f;
+  }
+#pragma unroll
+  for (int p = 0; p < MAPS; ++p)
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) first[p][i] = *reinterpret_cast<const f32x4*>(base + p * map + min(i * S + grp, splits - 1) * step + col);
+#pragma unroll
+  for (int p = 0; p < MAPS; ++p) {
+    float mm = m[p];
 #pragma unroll
     for (int d = 32; d; d >>= 1) mm = fmaxf(mm, __shfl_xor(mm, d));
-    const float w = m == -INFINITY ? 0.0f : exp2_(m - mm);
-    const float lt = wave_sum(w * l);
+    const float w = m[p] == -INFINITY ? 0.0f : exp2_(m[p] - mm);
+    const float lt = wave_sum(w * l[p]);
     f32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int s0 = 0; s0 < splits; s0 += S) {
-      const int s = s0 + grp;
-      const float ws = __shfl(w, min(s, 63));
-      if (s < splits) t += ws * *reinterpret_cast<const f32x4*>(base + s * step + col);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const float ws = __shfl(w, (i * S + grp) & 63);
+      if (i * S + grp < splits) t += ws * first[p][i];
+    }
+    for (int s0 = AHEAD * S; s0 < splits; s0 += S) {
+      const float ws = __shfl(w, (s0 + grp) & 63);
+      if (s0 + grp < splits) t += ws * *reinterpret_cast<const f32x4*>(base + p * map + (s0 + grp) * step + col);
     }
 #pragma unroll
     for (int d = C; d < 64; d <<= 1)
@@ -488,8 +511,6 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int splits, 
   }
   f32x4 x = y[0];
   if constexpr (MAPS == 2) {
-    float e1, e2;
-    const float lam = diff_lambda<TY>(a, e1, e2);
 #pragma unroll
     for (int r = 0; r < 4; ++r) x[r] = fmaf(-lam, y[1][r], x[r]);
   }
@@ -506,12 +527,21 @@ static bool is_step(const AttnArgs* a, bool bias) {
   const int G = a->H / a->Hkv;
   return (long)a->Lq * G <= 32 && (!bias || (long)G * (2 * (a->reach + BIAS_PAD) + 1) * 4 <= 16 * 1024);
 }
-// parts of at least 256 keys, no more than fill the chip four times
-static int step_splits(const AttnArgs* a) {
-  const long groups = (long)a->B * a->Hkv;
-  long s = (1024 + groups - 1) / groups, most = (a->Lk + 255) / 256;
+// Parts of at least 256 keys, and no more work-groups than the chip holds at a time (``resident`` a compute unit): a second round
+// would pay each work-group's start (lengths, first tile: ~4 us) again.
+static int step_splits(const AttnArgs* a, int resident) {
+  const long groups = (long)a->B * a->Hkv, most = (a->Lk + 255) / 256;
+  long s = (256 * resident + groups - 1) / groups;
   if (s > most) s = most;
   return s < 1 ? 1 : s > 64 ? 64 : (int)s;
+}
+template <typename L> static int step_lds(const AttnArgs* a, int tab) {
+  const int lds = L::LDS + a->H / a->Hkv * tab;
+  return lds > L::JOIN ? lds : L::JOIN;
+}
+template <typename L> static int step_resident(const AttnArgs* a, int tab) {
+  const int n = 160 * 1024 / step_lds<L>(a, tab);
+  return n < 1 ? 1 : n > 4 ? 4 : n;
 }
 
 template <int TY, int MAPS, int DQ, int DV, bool BIAS>
@@ -519,11 +549,11 @@ static int launch_fwd(const AttnArgs* a, hipStream_t stream) {
   constexpr int SZ = sizeof(typename El<TY>::T);
   const int tab = BIAS ? (2 * (a->reach + BIAS_PAD) + 1) * 4 : 0;
   if (is_step(a, BIAS)) {
-    const int splits = step_splits(a), G = a->H / a->Hkv;
+    typedef StepTile<TY, MAPS, DQ, DV> L;
+    const int splits = step_splits(a, step_resident<L>(a, tab)), G = a->H / a->Hkv;
     const long rows = (long)a->B * a->Hkv * MAPS * a->Lq * G;
     if (splits > 1 && (!a->ws || a->ws_floats < splits * rows * (DV + 4))) return SGTA_EBADARG;
-    typedef StepTile<TY, MAPS, DQ, DV> L;
-    const int lds = L::LDS + G * tab > L::JOIN ? L::LDS + G * tab : L::JOIN;
+    const int lds = step_lds<L>(a, tab);
     if (int e = allow_lds<attn_step_kernel<TY, MAPS, DQ, DV, BIAS>>(lds)) return e;
     hipLaunchKernelGGL((attn_step_kernel<TY, MAPS, DQ, DV, BIAS>), dim3(a->B * a->Hkv * splits), dim3(256), lds, stream, *a, splits);
     SGTA_LAUNCH_CHECK();
@@ -564,32 +594,32 @@ int attn_check(const AttnArgs* a, int maps) {
   return SGTA_OK;
 }
 
-extern "C" long sgta_attn_fwd_ws_floats(const sgta_attn_t* a, int maps) {
-  if ((maps != 1 && maps != 2) || attn_check(a, maps)) return 0;
-  if (!is_step(a, maps == 1)) return 0;
-  const int s = step_splits(a);
-  const int dv = maps == 1 ? pad_dim(a->Dv) : (a->D <= 32 && a->Dv <= 64 ? 64 : 128);
-  return s > 1 ? (long)s * a->B * a->H * maps * a->Lq * (dv + 4) : 0;
+// the variant for a call's types and sizes: launches it, or (ws) says how many floats of workspace it takes
+template <int TY, int MAPS, int DQ, int DV, bool BIAS> static int variant(const AttnArgs* a, hipStream_t st, long* ws) {
+  if (!ws) return launch_fwd<TY, MAPS, DQ, DV, BIAS>(a, st);
+  *ws = 0;
+  if (is_step(a, BIAS)) {
+    const int s = step_splits(a, step_resident<StepTile<TY, MAPS, DQ, DV>>(a, BIAS ? bias_size(a->reach) * 4 : 0));
+    if (s > 1) *ws = (long)s * a->B * a->H * MAPS * a->Lq * (DV + 4);
+  }
+  return SGTA_OK;
 }
-
-template <int TY> static int rel_fwd(const AttnArgs* a, hipStream_t st) {
+template <int TY> static int typed(const AttnArgs* a, int maps, hipStream_t st, long* ws) {
+  if (maps == 2) return a->D <= 32 && a->Dv <= 64 ? variant<TY, 2, 32, 64, false>(a, st, ws) : variant<TY, 2, 64, 128, false>(a, st, ws);
   switch (pad_dim(a->D)) {
-    case 32: return launch_fwd<TY, 1, 32, 32, true>(a, st);
-    case 64: return launch_fwd<TY, 1, 64, 64, true>(a, st);
-    default: return launch_fwd<TY, 1, 128, 128, true>(a, st);
+    case 32: return variant<TY, 1, 32, 32, true>(a, st, ws);
+    case 64: return variant<TY, 1, 64, 64, true>(a, st, ws);
+    default: return variant<TY, 1, 128, 128, true>(a, st, ws);
   }
 }
-template <int TY> static int diff_fwd(const AttnArgs* a, hipStream_t st) {
-  return a->D <= 32 && a->Dv <= 64 ? launch_fwd<TY, 2, 32, 64, false>(a, st) : launch_fwd<TY, 2, 64, 128, false>(a, st);
+static int forward(const AttnArgs* a, int maps, hipStream_t st, long* ws) {
+  if (int e = attn_check(a, maps)) return e;
+  return a->dtype == TY_F32 ? typed<TY_F32>(a, maps, st, ws) : a->dtype == TY_F16 ? typed<TY_F16>(a, maps, st, ws) : typed<TY_BF16>(a, maps, st, ws);
 }
 
-extern "C" int sgta_rel_attn_fwd(const sgta_attn_t* a, sgta_stream_t stream) {
-  if (int e = attn_check(a, 1)) return e;
-  hipStream_t st = (hipStream_t)stream;
-  return a->dtype == TY_F32 ? rel_fwd<TY_F32>(a, st) : a->dtype == TY_F16 ? rel_fwd<TY_F16>(a, st) : rel_fwd<TY_BF16>(a, st);
+extern "C" long sgta_attn_fwd_ws_floats(const sgta_attn_t* a, int maps) {
+  long n = 0;
+  return (maps == 1 || maps == 2) && forward(a, maps, nullptr, &n) == SGTA_OK ? n : 0;
 }
-extern "C" int sgta_diff_attn_fwd(const sgta_attn_t* a, sgta_stream_t stream) {
-  if (int e = attn_check(a, 2)) return e;
-  hipStream_t st = (hipStream_t)stream;
-  return a->dtype == TY_F32 ? diff_fwd<TY_F32>(a, st) : a->dtype == TY_F16 ? diff_fwd<TY_F16>(a, st) : diff_fwd<TY_BF16>(a, st);
-}
+extern "C" int sgta_rel_attn_fwd(const sgta_attn_t* a, sgta_stream_t stream) { return forward(a, 1, (hipStream_t)stream, nullptr); }
+extern "C" int sgta_diff_attn_fwd(const sgta_attn_t* a, sgta_stream_t stream) { return forward(a, 2, (hipStream_t)stream, nullptr); }

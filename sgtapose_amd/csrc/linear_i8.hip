@@ -16,7 +16,7 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 // that of the exact quotient: the remainder x - q xs is exact in one fma for the q next to it, and decides.
 template <int TY> __device__ __forceinline__ void load8(const typename El<TY>::T* p, int k, int K, bool vec, float (&v)[8]) {
   if (vec && k + 8 <= K) {
-    const typename El<TY>::Frag f = *reinterpret_cast<const typename El<TY>::Frag*>(p + k);
+    const typename El<TY>::Raw f = *reinterpret_cast<const typename El<TY>::Raw*>(p + k);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = (float)f[e];
   } else {

@@ -1,15 +1,16 @@
 """Attention with a bucketed relative bias and differential attention (sgtapose_amd/ops_attn.py) against the formulas in 64 bits.
 
 Tolerances are bounds, element by element, from the arithmetic of the kernels (u = eps / 2 of the element type, e = 2^-24):
-  scores    D products summed in f32, times the scale, plus the bias, minus the reference: off by at most
-            es = e ((D + 3) scale sum|q||k| + 4 |s| + 16), so a weight is off by a factor exp(2 es) (its own score and the sum's)
+  scores    D products summed in f32 (float operands as three bfloat16 numbers, whose smallest products, 3 e of |q||k|, are
+            left out), times the scale, plus the bias, minus the reference: off by at most
+            es = e ((D + 6) scale sum|q||k| + 4 |s| + 16), so a weight is off by a factor exp(2 es) (its own score and the sum's)
   weights   rounded to the element type before the product with v: u of each (IEEE half: 2^-25 at least, where it is subnormal)
-  sums      Lk terms in f32: e Lk of the sum of magnitudes
+  sums      Lk terms in f32: e (Lk + 3) of the sum of magnitudes
   output    rounded once more: u |o|
 Gradients, with a = 4 es + e Lk for the relative error of a weight from the saved statistics:
-  X = dO V^T   e (Dv + 2) |dO||V|^T;   delta: |dO| times the output's bound, and e (Dv + 2) |dO||O|
+  X = dO V^T   e (Dv + 5) |dO||V|^T;   delta: |dO| times the output's bound, and e (Dv + 2) |dO||O|
   dS           a |dS| + P (X's + delta's); rounded to the element type: u |dS| (IEEE half: scaled to |dO| next to one, so 2^-24 of it at least)
-  dQ, dK, dV   the sums of those errors times the other operand's magnitude, e per term of the sum, u of the result
+  dQ, dK, dV   the sums of those errors times the other operand's magnitude, e per term of the sum and 3 e, u of the result
 """
 import math
 
@@ -95,7 +96,7 @@ class Case:
             qp, kp = (q, k) if self.maps == 1 else (q[:, :, :, p], k[:, :, :, p])
             s = c * (qp @ kp.transpose(-1, -2)) + bias
             mag = c * (qp.abs() @ kp.abs().transpose(-1, -2))
-            es.append(E * ((D + 3) * mag + 4 * s.abs().clamp(max=1e4) + 16).amax((-1, -2), keepdim=True))
+            es.append(E * ((D + 6) * mag + 4 * s.abs().clamp(max=1e4) + 16).amax((-1, -2), keepdim=True))
             s = torch.where(seen, s, -math.inf)
             m = s.amax(-1, keepdim=True)
             e = torch.exp(s - torch.where(m == -math.inf, 0.0, m))
@@ -103,7 +104,7 @@ class Case:
             P.append(e / torch.where(t == 0, 1.0, t))
             qs.append(qp)
             ks.append(kp)
-        u, tiny, sums = U[T], FLUSH[T], Lk * E
+        u, tiny, sums = U[T], FLUSH[T], (Lk + 3) * E
         lam, lam_err = 0.0, 0.0
         if self.maps == 2:
             w = f(self.w)
@@ -128,7 +129,7 @@ def gradients(c):
     z = c.parts
     B, Lq, Lk, H, Hkv, D, Dv = c.dims
     G, u, P, v, do, lam = H // Hkv, z["u"], z["P"], z["v"], z["do"], z["lam"]
-    X, Xe = do @ v.transpose(-1, -2), E * (Dv + 2) * (do.abs() @ v.abs().transpose(-1, -2))
+    X, Xe = do @ v.transpose(-1, -2), E * (Dv + 5) * (do.abs() @ v.abs().transpose(-1, -2))
     top = do.abs().amax() * 2
     tiny = 2.0 ** -24 * top if c.dtype == torch.float16 else 0.0
     sgn = (1.0, -lam)
@@ -158,12 +159,12 @@ def gradients(c):
     dq, dk = [], []
     for p in range(c.maps):
         k, q, m = z["k"][p], z["q"][p], dS[p].abs()
-        e = Se[p] + (u + Lk * E) * m + tiny
+        e = Se[p] + (u + (Lk + 3) * E) * m + tiny
         dq.append((back(z["c"] * (dS[p] @ k)), back(z["c"] * (e @ k.abs()))))
-        e = Se[p] + (u + Lq * G * E) * m + tiny
+        e = Se[p] + (u + (Lq * G + 3) * E) * m + tiny
         dk.append((back(shared(z["c"] * (dS[p].transpose(-1, -2) @ q))), back(shared(z["c"] * (e.transpose(-1, -2) @ q.abs())))))
     w = sum(sgn[p] * P[p] for p in range(c.maps))
-    we = sum(abs(sgn[p]) * a[p] * P[p] for p in range(c.maps)) + (u + Lq * G * E) * sum(abs(sgn[p]) * P[p] for p in range(c.maps)) + z["tiny"]
+    we = sum(abs(sgn[p]) * a[p] * P[p] for p in range(c.maps)) + (u + (Lq * G + 3) * E) * sum(abs(sgn[p]) * P[p] for p in range(c.maps)) + z["tiny"]
     if c.maps == 2:
         we = we + 1e-5 * P[1]
     pack("dq", dq)
