@@ -101,34 +101,33 @@ struct I8Args {
   int M, N, K, relu, dtype;
 };
 
-// four consecutive channels n .. n + 3 of token m
-__device__ __forceinline__ void i8_store(const I8Args& a, int m, int n, i32x4 c, float xs) {
+// Four consecutive channels n .. n + 3 of token m.  WHOLE: all four exist (as 16 bytes of any row do) and are aligned.
+template <int TY, bool WHOLE> __device__ __forceinline__ void i8_store(const I8Args& a, int m, int n, i32x4 c, float xs) {
+  typedef typename El<TY>::T T;
+  T* o = (T*)a.out + (long)m * a.ldo + n;
+  const T* bias = (const T*)a.bias;
   f32x4 y;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    const int nn = min(n + r, a.N - 1);
-    float v = (float)c[r] * (xs * a.ws[nn]);
-    if (a.bias)
-      v += a.dtype == TY_F32 ? ((const float*)a.bias)[nn] : a.dtype == TY_F16 ? (float)((const _Float16*)a.bias)[nn] : (float)((const __bf16*)a.bias)[nn];
-    y[r] = a.relu ? (v < 0.0f ? 0.0f : v) : v;
+    const int nn = WHOLE ? n + r : min(n + r, a.N - 1);
+    y[r] = (float)c[r] * (xs * a.ws[nn]);
+    if (bias) y[r] += El<TY>::load(bias + nn);
+    if (a.relu) y[r] = y[r] < 0.0f ? 0.0f : y[r];
   }
-  const long at = (long)m * a.ldo + n;
-  const bool whole = n + 4 <= a.N && a.ldo % 4 == 0 && (uintptr_t)a.out % 16 == 0;
+  if (WHOLE) El<TY>::store4(o, y);
+  else
+    for (int r = 0; r < 4; ++r) if (n + r < a.N) El<TY>::store(o + r, y[r]);
+}
+// calls f<type, WHOLE> for the output at hand: one branch for all of a wave's stores
+template <typename F> __device__ __forceinline__ void i8_epilogue(const I8Args& a, F f) {
+  const int per = a.dtype == TY_F32 ? 4 : 8;
+  const bool whole = a.N % per == 0 && a.ldo % per == 0 && (uintptr_t)a.out % 16 == 0;
   if (a.dtype == TY_F32) {
-    float* o = (float*)a.out + at;
-    if (whole) El<TY_F32>::store4(o, y);
-    else
-      for (int r = 0; r < 4; ++r) if (n + r < a.N) El<TY_F32>::store(o + r, y[r]);
+    if (whole) f.template operator()<TY_F32, true>(); else f.template operator()<TY_F32, false>();
   } else if (a.dtype == TY_F16) {
-    _Float16* o = (_Float16*)a.out + at;
-    if (whole) El<TY_F16>::store4(o, y);
-    else
-      for (int r = 0; r < 4; ++r) if (n + r < a.N) El<TY_F16>::store(o + r, y[r]);
+    if (whole) f.template operator()<TY_F16, true>(); else f.template operator()<TY_F16, false>();
   } else {
-    __bf16* o = (__bf16*)a.out + at;
-    if (whole) El<TY_BF16>::store4(o, y);
-    else
-      for (int r = 0; r < 4; ++r) if (n + r < a.N) El<TY_BF16>::store(o + r, y[r]);
+    if (whole) f.template operator()<TY_BF16, true>(); else f.template operator()<TY_BF16, false>();
   }
 }
 
@@ -145,6 +144,75 @@ __device__ __forceinline__ i32x4 row16(const signed char* p, int k, int K) {
   }
   return v;
 }
+
+// A wave's accumulators: tokens m .. m + 32 MT, channels n .. n + 32 NN.  WHOLE: through a piece of LDS of the wave's own, 32 tokens
+// at a time, so that every store instruction writes 16-byte pieces of whole runs of a row.  (Straight from the registers a store
+// writes 16 bytes to each of 32 rows: at 16384 x 4096 x 4096 that took 130 of 380 us.)
+template <int MT, int NN> struct Finish {
+  const I8Args& a;
+  const i32x16 (&acc)[NN][MT];
+  int m, n;
+  char* lds;
+  static constexpr int PITCH = NN * 32 * 4 + 16, BYTES = 32 * PITCH;
+  template <int TY, bool WHOLE> __device__ __forceinline__ void operator()() const {
+    typedef typename El<TY>::T T;
+    const int lane = threadIdx.x & 63, li = lane & 31, half = lane >> 5;
+    if constexpr (!WHOLE) {
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        const int mm = m + 32 * j + li;
+        if (mm >= a.M) continue;
+        const float xs = a.xs[mm];
+#pragma unroll
+        for (int i = 0; i < NN; ++i)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int nn = n + 32 * i + 8 * g + 4 * half;
+            if (nn < a.N) i8_store<TY, false>(a, mm, nn, i32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]}, xs);
+          }
+      }
+    } else {
+      constexpr int SZ = sizeof(T), PER = NN * 32 * SZ / 16;       // 16-byte pieces of a row
+      f32x4 ws[NN][4], bias[NN][4];
+#pragma unroll
+      for (int i = 0; i < NN; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int nn = min(n + 32 * i + 8 * g + 4 * half, a.N - 4);
+          __builtin_memcpy(&ws[i][g], a.ws + nn, 16);
+          bias[i][g] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          if (a.bias)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) bias[i][g][r] = El<TY>::load((const T*)a.bias + nn + r);
+        }
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        const float xs = a.xs[min(m + 32 * j + li, a.M - 1)];
+        asm volatile("" ::: "memory");                 // a wave's LDS operations are done in order; the compiler keeps it
+#pragma unroll
+        for (int i = 0; i < NN; ++i)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            f32x4 y;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              y[r] = (float)acc[i][j][4 * g + r] * (xs * ws[i][g][r]) + bias[i][g][r];
+              if (a.relu) y[r] = y[r] < 0.0f ? 0.0f : y[r];
+            }
+            El<TY>::store4((T*)(lds + li * PITCH) + 32 * i + 8 * g + 4 * half, y);
+          }
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int p = 0; p < 32 * PER / 64; ++p) {
+          const int row = (p * 64 + lane) / PER, c = (p * 64 + lane) % PER;
+          const u32x4 v = *reinterpret_cast<const u32x4*>(lds + row * PITCH + c * 16);
+          const int mm = m + 32 * j + row, nn = n + c * (16 / SZ);
+          if (mm < a.M && nn < a.N) *reinterpret_cast<u32x4*>((T*)a.out + (long)mm * a.ldo + nn) = v;
+        }
+      }
+    }
+  }
+};
 
 // Tiled product: WM x WN waves, each (BM / WM) tokens x (BN / WN) channels in 32 x 32 tiles; 128-byte slices of k, double
 // buffered in LDS.  RAGGED false: rows of whole 16-byte pieces, copied straight into LDS (each lane's piece chosen so that the
@@ -257,20 +325,107 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_i8_kernel(I8Args a, int t
     if (s + 1 < slices) put((s & 1) ^ 1);
     __syncthreads();
   }
-#pragma unroll
-  for (int j = 0; j < MT; ++j) {
-    const int m = m0 + (wm * MT + j) * 32 + li;
-    if (m >= a.M) continue;
-    const float xs = a.xs[m];
-#pragma unroll
-    for (int i = 0; i < NN; ++i)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int n = n0 + (wn * NN + i) * 32 + 8 * g + 4 * half;
-        if (n < a.N) i8_store(a, m, n, i32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]}, xs);
-      }
-  }
+  static_assert(WM * WN * Finish<MT, NN>::BYTES <= 2 * STAGE, "the epilogue's pieces lie over the slices");
+  const Finish<MT, NN> fin{a, acc, m0 + wm * MT * 32, n0 + wn * NN * 32, smem + __builtin_amdgcn_readfirstlane(wave) * Finish<MT, NN>::BYTES};
+  i8_epilogue(a, fin);
 }
+
+// Large products: 256 x 256 tiles by 4 waves of 128 x 128, one a SIMD with its 512 registers.  LDS is what such a tile runs into
+// first: 4 waves read 8 fragments of 1 KB for 16 matrix instructions (256 of 512 cycles; 8 waves of 128 x 64: 384), and a quarter
+// more goes to filling it.  With one wave nothing else hides a wait, so everything is fetched ahead: the next 128-byte slice of k
+// (whole cache lines of every row) into the other buffer from the last of a slice's four steps on, and the next step's fragments
+// into the other set of registers, also across the slices' one barrier, which comes before the last step's products.
+__global__ __launch_bounds__(256, 1) void linear_i8_large_kernel(I8Args a, int tm, int tn) {
+  constexpr int STAGE = 512 * 128;                                // 256 token rows, then 256 channel rows
+  extern __shared__ __align__(16) char smem[];
+  const int T = tm * tn, per = (T + 7) / 8, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || id >= T) return;
+  const int g0 = id / (8 * tn) * 8, gm = min(8, tm - g0), rest = id - g0 * tn;
+  const int m0 = (g0 + rest % gm) * 256, n0 = rest / gm * 256;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, half = lane >> 5;
+  const int wm = wave & 1, wn = wave >> 1;
+  const int slices = (a.K + 127) / 128;
+  const int xrows = min(256, a.M - m0), wrows = min(256, a.N - n0);
+  // piece 256 i + tid: row 32 i + tid / 8, 16-byte piece (tid ^ row) & 7 of the slice, stored at its place
+  const int r0 = tid >> 3, ch = ((tid ^ r0) & 7) * 16;
+  unsigned xoff = r0 * (int)a.ldx + ch, woff = r0 * (int)a.ldw + ch;
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef __attribute__((address_space(3))) void* lds_ptr_t;
+  const unsigned lds0 = (unsigned)(size_t)(lds_ptr_t)(smem + wave * 1024);
+  const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<signed char*>(a.xq + (long)m0 * a.ldx), (short)0, (int)((xrows - 1) * a.ldx + a.K), 0x00020000);
+  const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(const_cast<signed char*>(a.wq + (long)n0 * a.ldw), (short)0, (int)((wrows - 1) * a.ldw + a.K), 0x00020000);
+#endif
+  // one of a slice's sixteen loads of this wave; rows beyond the last lie beyond the resource: zeros
+  auto fetch = [&](int s, int i) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const int at = s * 128;
+    const bool in = at + ch < a.K;                                // the last slice may be a part of one; those behind it are none
+    const int step = 32 * (i & 7), ld = (int)(i < 8 ? a.ldx : a.ldw);
+    dma16(i < 8 ? xr : wr, in ? (i < 8 ? xoff : woff) + (unsigned)(step * ld + at) : 0x80000000u, lds0 + (s & 1) * STAGE + i * 4096);
+#endif
+  };
+  const char* xb = smem + (wm * 128 + li) * 128;
+  const char* wb = smem + (256 + wn * 128 + li) * 128;
+  auto read = [&](i32x4 (&wf)[4], i32x4 (&xf)[4], int s, int k) {
+    const int at = (s & 1) * STAGE + (((2 * k + half) ^ li) & 7) * 16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) wf[i] = *reinterpret_cast<const i32x4*>(wb + at + i * 4096);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) xf[i] = *reinterpret_cast<const i32x4*>(xb + at + i * 4096);
+  };
+  i32x16 acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = i32x16{0};
+  i32x4 wf[2][4], xf[2][4];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) fetch(0, i);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) fetch(1, i);
+  dma_wait<8>();
+  __syncthreads();
+  read(wf[0], xf[0], 0, 0);
+  for (int s = 0; s < slices; ++s) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (k == 3) {
+        dma_wait<0>();                                            // the next slice has landed,
+        __builtin_amdgcn_s_waitcnt(0xc07f);                       // this one is in registers,
+        __builtin_amdgcn_s_barrier();                             // for every wave
+      }
+      // the next step's fragments first (the scheduler would put each read next to its use), this step's products under them
+      if (k < 3) read(wf[(k + 1) & 1], xf[(k + 1) & 1], s, k + 1);
+      else read(wf[0], xf[0], s + 1, 0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[k & 1][i], xf[k & 1][j], acc[i][j], 0, 0, 0);
+        if (k == 0) {
+          fetch(s + 1, 8 + 2 * i);
+          fetch(s + 1, 9 + 2 * i);
+        }
+        if (k == 3) {
+          fetch(s + 2, 2 * i);
+          fetch(s + 2, 2 * i + 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+  dma_wait<0>();
+  __syncthreads();                                                // the epilogue's pieces lie over the slices
+  const Finish<4, 4> fin{a, acc, m0 + wm * 128, n0 + wn * 128, smem + wave * Finish<4, 4>::BYTES};
+  i8_epilogue(a, fin);
+}
+
+struct FinishOne {
+  const I8Args& a;
+  int m, n;
+  i32x4 c;
+  template <int TY, bool WHOLE> __device__ __forceinline__ void operator()() const { i8_store<TY, WHOLE>(a, m, n, c, a.xs[m]); }
+};
 
 // Few tokens: the weights are read once, straight into registers.  A work-group has 16 channels and up to 16 MT tokens
 // (blockIdx.y: the next 16 MT); its 16 waves share k in pieces of 64 bytes and are summed in LDS.
@@ -321,7 +476,7 @@ __global__ __launch_bounds__(1024) void linear_i8_few_kernel(I8Args a) {
 #pragma unroll
   for (int v = 1; v < 16; ++v) c += part[v][wave][lane];
   const int m = m0 + 16 * wave + li, n = n0 + 4 * q;
-  if (m < a.M && n < a.N) i8_store(a, m, n, c, a.xs[m]);
+  if (m < a.M && n < a.N) i8_epilogue(a, FinishOne{a, m, n, c});
 }
 
 template <int BM, int BN, int WM, int WN, bool RAGGED> static int launch_i8(const I8Args& a, hipStream_t st) {
@@ -329,6 +484,14 @@ template <int BM, int BN, int WM, int WN, bool RAGGED> static int launch_i8(cons
   if ((long)tm * tn > 0x7ffffff0L) return SGTA_ETOOBIG;
   if (int e = allow_lds<linear_i8_kernel<BM, BN, WM, WN, RAGGED>>(lds)) return e;
   hipLaunchKernelGGL((linear_i8_kernel<BM, BN, WM, WN, RAGGED>), dim3((tm * tn + 7) / 8 * 8), dim3(64 * WM * WN), lds, st, a, tm, tn);
+  SGTA_LAUNCH_CHECK();
+  return SGTA_OK;
+}
+static int launch_i8_large(const I8Args& a, hipStream_t st) {
+  const int tm = cdiv(a.M, 256), tn = cdiv(a.N, 256), lds = 2 * 512 * 128;
+  if ((long)tm * tn > 0x7ffffff0L) return SGTA_ETOOBIG;
+  if (int e = allow_lds<linear_i8_large_kernel>(lds)) return e;
+  hipLaunchKernelGGL(linear_i8_large_kernel, dim3((tm * tn + 7) / 8 * 8), dim3(256), lds, st, a, tm, tn);
   SGTA_LAUNCH_CHECK();
   return SGTA_OK;
 }
@@ -362,7 +525,7 @@ extern "C" int sgta_linear_i8(const signed char* xq, long ldx, const float* xs, 
     return ragged ? launch_few<4, true>(a, st) : launch_few<4, false>(a, st);
   }
   // the largest tile that still gives most of the 256 compute units one
-  if (!ragged && (long)cdiv(M, 256) * cdiv(N, 256) >= 192) return launch_i8<256, 256, 2, 4, false>(a, st);
+  if (!ragged && (long)cdiv(M, 256) * cdiv(N, 256) >= 192) return launch_i8_large(a, st);
   if ((long)cdiv(M, 128) * cdiv(N, 128) >= 192) return ragged ? launch_i8<128, 128, 2, 2, true>(a, st) : launch_i8<128, 128, 2, 2, false>(a, st);
   return ragged ? launch_i8<64, 64, 2, 2, true>(a, st) : launch_i8<64, 64, 2, 2, false>(a, st);
 }
