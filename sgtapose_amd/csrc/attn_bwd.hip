@@ -29,9 +29,10 @@ __device__ __forceinline__ float pow2_to_one(float top) {          // 2^-exponen
 struct BwdWork {
   long delta, part, top;       // [maps][B][H][Lq]; per (b, h, query block): sums by bucket, or of d2; largest |dO|
   long total;
-  int nblk, nsum, nrel;        // query blocks; floats of a part; distances a work-group tells apart
+  int rw, nblk, nsum, nrel;    // attn_dq_kernel's waves by rows and query blocks; floats of a part; distances told apart
   __host__ __device__ BwdWork(const AttnArgs& a, int maps) {
-    nblk = (a.Lq + 127) / 128;
+    rw = row_waves((long)a.B * a.H * ((a.Lq + 127) / 128));
+    nblk = (a.Lq + 32 * rw - 1) / (32 * rw);
     nrel = 2 * (a.reach + BIAS_PAD) + 1;
     nsum = maps == 1 ? a.num_buckets : 1;
     const long blocks = (long)a.B * a.H * nblk;
@@ -42,11 +43,11 @@ struct BwdWork {
   }
 };
 
-template <int TY, int MAPS, int DQ, int DV, bool BIAS>
+template <int TY, int MAPS, int DQ, int DV, bool BIAS, int RW>
 __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2) void attn_dq_kernel(AttnArgs a) {
   typedef typename El<TY>::T T;
   typedef typename El<TY>::Frag Frag;
-  constexpr int KT = TY == TY_F32 ? 32 : 64;
+  constexpr int KT = TY == TY_F32 && RW == 4 ? 32 : 64;
   typedef Tile<TY, DQ> TK;
   typedef Tile<TY, DV> TV;
   constexpr int MB = KT * TK::ROWB, KB = MAPS * MB, VB = KT * TV::ROWB;
@@ -58,7 +59,7 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
   const int bh = blockIdx.x % (a.B * a.H), b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
   const int blk = a.causal ? nblk - 1 - blockIdx.x / (a.B * a.H) : blockIdx.x / (a.B * a.H);
   const int nq = clamp_len(a.q_len, b, a.Lq), nk = clamp_len(a.kv_len, b, a.Lk), st = start_of(a.q_start, b);
-  const int blk0 = blk * 128;
+  const int blk0 = blk * 32 * RW, half_of = RW == 2 ? wave >> 1 : 0;         // rows; which half of each tile's keys
   float* part = a.ws + wk.part + ((long)bh * nblk + blk) * wk.nsum;
   float* topw = a.ws + wk.top + (long)bh * nblk + blk;
   if (blk0 >= nq) {
@@ -66,9 +67,9 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
     if (tid == 0) *topw = 0.0f;
     return;
   }
-  const int row0 = blk0 + wave * 32, row = row0 + li;
+  const int row0 = blk0 + (RW == 2 ? wave & 1 : wave) * 32, row = row0 + li;
   const bool ok = row < nq;
-  const int last_row = min(blk0 + 127, nq - 1);
+  const int last_row = min(blk0 + 32 * RW - 1, nq - 1);
   const int seen = a.causal ? min(nk, max(st + last_row + 1, 0)) : nk;
   const int nt = (seen + KT - 1) / KT;
   const T* kp = (const T*)a.k + b * a.sk[0] + hk * a.sk[2];
@@ -147,7 +148,7 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
     if (tid == 0) *topw = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     if constexpr (MAPS == 2) {
       __syncthreads();
-      const float t2 = wave_sum(half == 0 && ok ? dl[1] : 0.0f);
+      const float t2 = wave_sum(half == 0 && half_of == 0 && ok ? dl[1] : 0.0f);
       if (lane == 0) red[wave] = t2;
       __syncthreads();
       if (tid == 0) part[0] = (red[0] + red[1]) + (red[2] + red[3]);
@@ -192,7 +193,7 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
 #pragma unroll
     for (int u = 0; u < KT / 32; ++u) {
       const int j0 = t * KT + 32 * u;
-      if (j0 > wave_last) continue;
+      if (j0 > wave_last || (RW == 2 && u != half_of)) continue;
       const bool masked = low < j0 + 31;
       const bool left = BIAS && j0 + 31 - pmin <= -a.reach, right = BIAS && j0 - pmax >= a.reach;
       const bool plain = !masked && (!BIAS || (fold && (left || right)));
@@ -281,7 +282,32 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
     __syncthreads();
   }
 
-  if (ok) {
+  float e = half_sum((sum_l + sum_r) + sum_n);                       // of a row's dS over all its keys
+  if constexpr (RW == 2) {
+    // the second half's sums, register by register, over the tiles: every wave is past its last read
+    float* y = reinterpret_cast<float*>(smem) + (wave & 1) * 64 + lane;
+    float* z = reinterpret_cast<float*>(smem) + MAPS * DQ / 2 * 128 + (wave & 1) * 128 + half_of * 64 + lane;
+    if (half_of == 1) {
+#pragma unroll
+      for (int p = 0; p < MAPS; ++p)
+#pragma unroll
+        for (int d = 0; d < DQ / 32; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) y[((p * (DQ / 32) + d) * 16 + r) * 128] = dq[p][d][r];
+    }
+    if (BIAS) z[0] = e;
+    __syncthreads();
+    if (half_of == 0) {
+#pragma unroll
+      for (int p = 0; p < MAPS; ++p)
+#pragma unroll
+        for (int d = 0; d < DQ / 32; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dq[p][d][r] += y[((p * (DQ / 32) + d) * 16 + r) * 128];
+    }
+    if (BIAS) e += z[half_of ? -64 : 64];
+  }
+  if (ok && half_of == 0) {
     T* o = (T*)a.dq + b * a.sdq[0] + row * a.sdq[1] + h * a.sdq[2];
     const float f = a.scale * irs;
 #pragma unroll
@@ -298,7 +324,6 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
   if constexpr (BIAS) {
     // A row's dS sums to zero, but for delta's error (it comes from an output that was rounded): of the far buckets, where P's
     // sum is large, that error times the sum is taken off again.
-    const float e = half_sum((sum_l + sum_r) + sum_n);
     sum_l = wave_sum(ok ? fmaf(-e, p_l, sum_l) : 0.0f);
     sum_r = wave_sum(ok ? fmaf(-e, p_r, sum_r) : 0.0f);
     if (lane == 0) {                                  // the ends of the table stand for everything beyond
@@ -326,7 +351,7 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
   }
 }
 
-template <int TY, int MAPS, int DQ, int DV, bool BIAS>
+template <int TY, int MAPS, int DQ, int DV, bool BIAS, int RW>
 __global__ __launch_bounds__(256, (MAPS * DQ + DV > 128 || (TY == TY_F32 && MAPS * DQ + DV > 64)) ? 1 : 2) void attn_dkv_kernel(AttnArgs a, int nblk) {
   typedef typename El<TY>::T T;
   typedef typename El<TY>::Frag Frag;
@@ -341,9 +366,9 @@ __global__ __launch_bounds__(256, (MAPS * DQ + DV > 128 || (TY == TY_F32 && MAPS
   const int bh = blockIdx.x % (a.B * a.Hkv), b = bh / a.Hkv, hk = bh % a.Hkv, blk = blockIdx.x / (a.B * a.Hkv);
   const int G = a.H / a.Hkv;
   const int nq = clamp_len(a.q_len, b, a.Lq), nk = clamp_len(a.kv_len, b, a.Lk), st = start_of(a.q_start, b);
-  const int blk0 = blk * 128;
+  const int blk0 = blk * 32 * RW, half_of = RW == 2 ? wave >> 1 : 0;         // keys; which half of each tile's queries
   if (blk0 >= nk) return;
-  const int key0 = blk0 + wave * 32, key = key0 + li;
+  const int key0 = blk0 + (RW == 2 ? wave & 1 : wave) * 32, key = key0 + li;
   const bool ok = key < nk;
   const float c2 = a.scale * LOG2E, ic2 = 1.0f / c2;
   const bool both = a.D > 16;                         // DQ = 32: the second 16 of the head's elements are not all padding
@@ -448,7 +473,7 @@ __global__ __launch_bounds__(256, (MAPS * DQ + DV > 128 || (TY == TY_F32 && MAPS
 #pragma unroll 1
     for (int u = 0; u < QT / 32; ++u) {
       const int q0 = r0 + 32 * u;
-      if (q0 + 31 < wave_first || q0 >= nq) continue;
+      if (q0 + 31 < wave_first || q0 >= nq || (RW == 2 && u != half_of)) continue;
       const bool diag = a.causal && q0 < key0 + 31 - st;             // some pair of the tile is masked
       const bool left = BIAS && key0 + 31 - (st + q0) <= -a.reach, right = BIAS && key0 - (st + q0 + 31) >= a.reach;
       const bool plain = !diag && (!BIAS || (fold && (left || right)));
@@ -539,6 +564,34 @@ __global__ __launch_bounds__(256, (MAPS * DQ + DV > 128 || (TY == TY_F32 && MAPS
     dma_wait<0>();
     __syncthreads();
   }
+  if constexpr (RW == 2) {
+    // the second half's sums, register by register, over the tiles: every wave is past its last read
+    float* y = reinterpret_cast<float*>(smem) + (wave & 1) * 64 + lane;
+    if (half_of == 1) {
+#pragma unroll
+      for (int p = 0; p < MAPS; ++p)
+#pragma unroll
+        for (int d = 0; d < DQ / 32; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) y[((p * (DQ / 32) + d) * 16 + r) * 128] = dk[p][d][r];
+#pragma unroll
+      for (int d = 0; d < DV / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) y[((MAPS * (DQ / 32) + d) * 16 + r) * 128] = dv[d][r];
+    }
+    __syncthreads();
+    if (half_of == 1) return;
+#pragma unroll
+    for (int p = 0; p < MAPS; ++p)
+#pragma unroll
+      for (int d = 0; d < DQ / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dk[p][d][r] += y[((p * (DQ / 32) + d) * 16 + r) * 128];
+#pragma unroll
+    for (int d = 0; d < DV / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dv[d][r] += y[((MAPS * (DQ / 32) + d) * 16 + r) * 128];
+  }
   if (!ok) return;
   T* ko = (T*)a.dk + b * a.sdk[0] + key * a.sdk[1] + hk * a.sdk[2];
   T* vo = (T*)a.dv + b * a.sdv[0] + key * a.sdv[1] + hk * a.sdv[2];
@@ -606,20 +659,31 @@ __global__ __launch_bounds__(256) void diff_dw_kernel(AttnArgs a) {
   }
 }
 
+static inline int at_least(int a, int b) { return a > b ? a : b; }
+template <int TY, int MAPS, int DQ, int DV, bool BIAS, int RW> static int launch_dq(const AttnArgs* a, const BwdWork& wk, hipStream_t stream) {
+  constexpr int KT = TY == TY_F32 && RW == 4 ? 32 : 64, STAGE = 2 * KT * (MAPS * DQ + DV) * (int)sizeof(typename El<TY>::T);
+  constexpr int JOIN = RW == 2 ? (MAPS * DQ / 2 + 2) * 128 * 4 : 0;
+  static_assert(JOIN <= STAGE, "the halves' sums lie over the tiles");
+  const int lds = STAGE + (BIAS ? (5 * wk.nrel + 4 * DIAG) * 4 : 0);
+  if (int e = allow_lds<attn_dq_kernel<TY, MAPS, DQ, DV, BIAS, RW>>(lds)) return e;
+  hipLaunchKernelGGL((attn_dq_kernel<TY, MAPS, DQ, DV, BIAS, RW>), dim3(a->B * a->H * wk.nblk), dim3(256), lds, stream, *a);
+  SGTA_LAUNCH_CHECK();
+  return SGTA_OK;
+}
+template <int TY, int MAPS, int DQ, int DV, bool BIAS, int RW> static int launch_dkv(const AttnArgs* a, const BwdWork& wk, hipStream_t stream) {
+  constexpr int STAGE = 2 * (64 * (MAPS * DQ + DV) * (int)sizeof(typename El<TY>::T) + 4 * MAPS * 64 * 4);
+  constexpr int JOIN = RW == 2 ? (MAPS * DQ + DV) / 2 * 128 * 4 : 0;
+  const int nblk = cdiv(a->Lk, 32 * RW), lds = at_least(STAGE + (BIAS ? wk.nrel * 4 : 0), JOIN);
+  if (int e = allow_lds<attn_dkv_kernel<TY, MAPS, DQ, DV, BIAS, RW>>(lds)) return e;
+  hipLaunchKernelGGL((attn_dkv_kernel<TY, MAPS, DQ, DV, BIAS, RW>), dim3(a->B * a->Hkv * nblk), dim3(256), lds, stream, *a, nblk);
+  SGTA_LAUNCH_CHECK();
+  return SGTA_OK;
+}
 template <int TY, int MAPS, int DQ, int DV, bool BIAS> static int launch_bwd(const AttnArgs* a, hipStream_t stream) {
-  constexpr int SZ = sizeof(typename El<TY>::T);
   const BwdWork wk(*a, MAPS);
-  const int tab = BIAS ? wk.nrel * 4 : 0;
-  constexpr int KT = TY == TY_F32 ? 32 : 64;
-  int lds = 2 * KT * (MAPS * DQ + DV) * SZ + 5 * tab + (BIAS ? 4 * DIAG * 4 : 0);
-  if (int e = allow_lds<attn_dq_kernel<TY, MAPS, DQ, DV, BIAS>>(lds)) return e;
-  hipLaunchKernelGGL((attn_dq_kernel<TY, MAPS, DQ, DV, BIAS>), dim3(a->B * a->H * wk.nblk), dim3(256), lds, stream, *a);
-  SGTA_LAUNCH_CHECK();
-  const int nblk = cdiv(a->Lk, 128);
-  lds = 2 * (64 * (MAPS * DQ + DV) * SZ + 4 * MAPS * 64 * 4) + tab;
-  if (int e = allow_lds<attn_dkv_kernel<TY, MAPS, DQ, DV, BIAS>>(lds)) return e;
-  hipLaunchKernelGGL((attn_dkv_kernel<TY, MAPS, DQ, DV, BIAS>), dim3(a->B * a->Hkv * nblk), dim3(256), lds, stream, *a, nblk);
-  SGTA_LAUNCH_CHECK();
+  if (int e = wk.rw == 2 ? launch_dq<TY, MAPS, DQ, DV, BIAS, 2>(a, wk, stream) : launch_dq<TY, MAPS, DQ, DV, BIAS, 4>(a, wk, stream)) return e;
+  const bool two = row_waves((long)a->B * a->Hkv * cdiv(a->Lk, 128)) == 2;
+  if (int e = two ? launch_dkv<TY, MAPS, DQ, DV, BIAS, 2>(a, wk, stream) : launch_dkv<TY, MAPS, DQ, DV, BIAS, 4>(a, wk, stream)) return e;
   if (MAPS == 1) hipLaunchKernelGGL((rel_dw_kernel<TY>), dim3(a->H * a->num_buckets), dim3(256), 0, stream, *a);
   else hipLaunchKernelGGL((diff_dw_kernel<TY>), dim3(1), dim3(256), 0, stream, *a);
   SGTA_LAUNCH_CHECK();

@@ -167,10 +167,13 @@ __device__ __forceinline__ FwdPlace fwd_place(const AttnArgs& a, int nblk) {
   return w;
 }
 
-template <int TY, int MAPS, int DQ, int DV, bool BIAS>
-__global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a, int nblk) {
+// RW: waves by rows (4, or 2 with two waves a row, see row_waves)
+template <int TY, int RW> struct KeyTile { static constexpr int KT = TY == TY_F32 && RW == 4 ? 32 : 64; };   // keys staged at a time
+
+template <int TY, int MAPS, int DQ, int DV, bool BIAS, int RW>
+__global__ __launch_bounds__(256, TY == TY_F32 && MAPS * DQ + DV > 128 ? 1 : 2) void attn_fwd_kernel(AttnArgs a, int nblk) {
   typedef typename El<TY>::T T;
-  constexpr int KT = TY == TY_F32 ? 32 : 64, NK = TY == TY_F32 || (MAPS == 2 && DV > 64) ? 32 : 64;   // keys staged; keys at a time
+  constexpr int KT = KeyTile<TY, RW>::KT, NK = RW == 2 || TY == TY_F32 || (MAPS == 2 && DV > 64) ? 32 : 64;   // keys at a time
   constexpr int MB = KT * DQ * (int)sizeof(T), KB = MAPS * MB, VB = KT * DV * (int)sizeof(T);
   extern __shared__ __align__(16) char smem[];       // 2 x (K maps, V), then the bias table
   float* tab = reinterpret_cast<float*>(smem + 2 * (KB + VB));
@@ -179,10 +182,10 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a, int nblk) 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, half = lane >> 5;
   const int b = w.b, h = w.h, hk = h / (a.H / a.Hkv);
   const int nq = clamp_len(a.q_len, b, a.Lq), nk = clamp_len(a.kv_len, b, a.Lk), st = start_of(a.q_start, b);
-  const int blk0 = w.blk * 128;
+  const int blk0 = w.blk * 32 * RW, part = RW == 2 ? wave >> 1 : 0;          // rows; which half of each tile's keys
   if (blk0 >= nq) return;
-  const int row0 = blk0 + wave * 32, row = row0 + li;
-  const int last_row = min(blk0 + 127, nq - 1);
+  const int row0 = blk0 + (RW == 2 ? wave & 1 : wave) * 32, row = row0 + li;
+  const int last_row = min(blk0 + 32 * RW - 1, nq - 1);
   const int seen = a.causal ? min(nk, max(st + last_row + 1, 0)) : nk;      // keys any row of this block sees
   const int nt = (seen + KT - 1) / KT;
 
@@ -226,11 +229,41 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a, int nblk) 
     if (t + 1 < nt) fetch((t + 1) * KT, (t & 1) ^ 1);
 #pragma unroll
     for (int u = 0; u < KT / NK; ++u)
-      if (t * KT + u * NK <= wave_last) wv.template step<NK>(kt, MB, kt + KB, u * NK, t * KT + u * NK, a.reach, lane);
+      if ((RW == 4 || u == part) && t * KT + u * NK <= wave_last) wv.template step<NK>(kt, MB, kt + KB, u * NK, t * KT + u * NK, a.reach, lane);
     dma_wait<0>();
     __syncthreads();
   }
 
+  if constexpr (RW == 2) {
+    // the second half's state, register by register, over the tiles: every wave is past its last read
+    float* x = reinterpret_cast<float*>(smem) + (wave & 1) * 64 + lane;
+    if (part == 1) {
+#pragma unroll
+      for (int p = 0; p < MAPS; ++p) {
+        float* y = x + p * (DV / 2 + 2) * 128;
+        y[0] = wv.m[p];
+        y[128] = wv.l[p];
+#pragma unroll
+        for (int d = 0; d < DV / 32; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) y[(2 + 16 * d + r) * 128] = wv.o[p][d][r];
+      }
+    }
+    __syncthreads();
+    if (part == 1) return;
+#pragma unroll
+    for (int p = 0; p < MAPS; ++p) {
+      const float* y = x + p * (DV / 2 + 2) * 128;
+      const float m2 = y[0], mm = fmaxf(wv.m[p], m2);
+      const float w1 = wv.m[p] == -INFINITY ? 0.0f : exp2_(wv.m[p] - mm), w2 = m2 == -INFINITY ? 0.0f : exp2_(m2 - mm);
+      wv.m[p] = mm;
+      wv.l[p] = fmaf(wv.l[p], w1, y[128] * w2);
+#pragma unroll
+      for (int d = 0; d < DV / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) wv.o[p][d][r] = fmaf(wv.o[p][d][r], w1, y[(2 + 16 * d + r) * 128] * w2);
+    }
+  }
   float lam = 0.0f;
   if constexpr (MAPS == 2) {
     float e1, e2;
@@ -544,9 +577,16 @@ template <typename L> static int step_resident(const AttnArgs* a, int tab) {
   return n < 1 ? 1 : n > 4 ? 4 : n;
 }
 
+template <int TY, int MAPS, int DQ, int DV, bool BIAS, int RW> static int launch_rows(const AttnArgs* a, int tab, hipStream_t stream) {
+  constexpr int STAGE = 2 * KeyTile<TY, RW>::KT * (MAPS * DQ + DV) * (int)sizeof(typename El<TY>::T), JOIN = MAPS * (DV / 2 + 2) * 128 * 4;
+  const int lds = (RW == 2 && JOIN > STAGE ? JOIN : STAGE) + tab, nblk = cdiv(a->Lq, 32 * RW);
+  if (int e = allow_lds<attn_fwd_kernel<TY, MAPS, DQ, DV, BIAS, RW>>(lds)) return e;
+  hipLaunchKernelGGL((attn_fwd_kernel<TY, MAPS, DQ, DV, BIAS, RW>), dim3(a->B * a->H * nblk), dim3(256), lds, stream, *a, nblk);
+  SGTA_LAUNCH_CHECK();
+  return SGTA_OK;
+}
 template <int TY, int MAPS, int DQ, int DV, bool BIAS>
 static int launch_fwd(const AttnArgs* a, hipStream_t stream) {
-  constexpr int SZ = sizeof(typename El<TY>::T);
   const int tab = BIAS ? (2 * (a->reach + BIAS_PAD) + 1) * 4 : 0;
   if (is_step(a, BIAS)) {
     typedef StepTile<TY, MAPS, DQ, DV> L;
@@ -564,13 +604,8 @@ static int launch_fwd(const AttnArgs* a, hipStream_t stream) {
     }
     return SGTA_OK;
   }
-  constexpr int KT = TY == TY_F32 ? 32 : 64;
-  const int lds = 2 * KT * (MAPS * DQ + DV) * SZ + tab;
-  const int nblk = cdiv(a->Lq, 128);
-  if (int e = allow_lds<attn_fwd_kernel<TY, MAPS, DQ, DV, BIAS>>(lds)) return e;
-  hipLaunchKernelGGL((attn_fwd_kernel<TY, MAPS, DQ, DV, BIAS>), dim3(a->B * a->H * nblk), dim3(256), lds, stream, *a, nblk);
-  SGTA_LAUNCH_CHECK();
-  return SGTA_OK;
+  return row_waves((long)a->B * a->H * cdiv(a->Lq, 128)) == 2 ? launch_rows<TY, MAPS, DQ, DV, BIAS, 2>(a, tab, stream)
+                                                              : launch_rows<TY, MAPS, DQ, DV, BIAS, 4>(a, tab, stream);
 }
 
 // what both directions refuse
