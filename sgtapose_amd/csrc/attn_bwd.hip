@@ -43,17 +43,24 @@ struct BwdWork {
   }
 };
 
+// LDS of attn_dq_kernel before the bias table: two stages of keys, or what lies over them at the end
+template <int TY, int MAPS, int DQ, int DV, int RW> struct DqLds {
+  static constexpr int KT = TY == TY_F32 && RW == 4 ? 32 : 64, STAGE = 2 * KT * (MAPS * DQ + DV) * (int)sizeof(typename El<TY>::T);
+  static constexpr int JOIN = RW == 2 ? (MAPS * DQ / 2 + 2) * 128 * 4 : 0, OUT = 4 * RowStore<TY, DQ>::BYTES;
+  static constexpr int ALL = OUT > STAGE ? OUT : STAGE;
+  static_assert(JOIN <= STAGE, "the halves' sums lie over the tiles");
+};
 template <int TY, int MAPS, int DQ, int DV, bool BIAS, int RW>
 __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2) void attn_dq_kernel(AttnArgs a) {
   typedef typename El<TY>::T T;
   typedef typename El<TY>::Frag Frag;
-  constexpr int KT = TY == TY_F32 && RW == 4 ? 32 : 64;
+  constexpr int KT = DqLds<TY, MAPS, DQ, DV, RW>::KT;
   typedef Tile<TY, DQ> TK;
   typedef Tile<TY, DV> TV;
   constexpr int MB = KT * TK::ROWB, KB = MAPS * MB, VB = KT * TV::ROWB;
   extern __shared__ __align__(16) char smem[];       // 2 x (K maps, V) | bias table | 4 waves: sums by distance | 4 waves: DIAG
   const BwdWork wk(a, MAPS);
-  float* tab = reinterpret_cast<float*>(smem + 2 * (KB + VB));
+  float* tab = reinterpret_cast<float*>(smem + DqLds<TY, MAPS, DQ, DV, RW>::ALL);
   __shared__ float red[4];
   const int nblk = wk.nblk, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, half = lane >> 5;
   const int bh = blockIdx.x % (a.B * a.H), b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
@@ -307,19 +314,12 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
     }
     if (BIAS) e += z[half_of ? -64 : 64];
   }
-  if (ok && half_of == 0) {
-    T* o = (T*)a.dq + b * a.sdq[0] + row * a.sdq[1] + h * a.sdq[2];
-    const float f = a.scale * irs;
+  typedef RowStore<TY, DQ> Out;
+  if (RW == 2) __syncthreads();                                      // past the join's reads
+  if (row0 < nq && half_of == 0) {
+    T* o = (T*)a.dq + b * a.sdq[0] + row0 * a.sdq[1] + h * a.sdq[2];
 #pragma unroll
-    for (int p = 0; p < MAPS; ++p)
-#pragma unroll
-      for (int d = 0; d < DQ / 32; ++d)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int col = 32 * d + 8 * c + 4 * half;
-          f32x4 y = {dq[p][d][4 * c] * f, dq[p][d][4 * c + 1] * f, dq[p][d][4 * c + 2] * f, dq[p][d][4 * c + 3] * f};
-          if (col < a.D) El<TY>::store4(o + (MAPS == 2 ? p * a.sdq[3] : 0) + col, y);
-        }
+    for (int p = 0; p < MAPS; ++p) Out::store(dq[p], a.scale * irs, smem + wave * Out::BYTES, o + (MAPS == 2 ? p * a.sdq[3] : 0), a.sdq[1], nq - row0, a.D, lane);
   }
   if constexpr (BIAS) {
     // A row's dS sums to zero, but for delta's error (it comes from an output that was rounded): of the far buckets, where P's
@@ -580,39 +580,30 @@ __global__ __launch_bounds__(256, (MAPS * DQ + DV > 128 || (TY == TY_F32 && MAPS
         for (int r = 0; r < 16; ++r) y[((MAPS * (DQ / 32) + d) * 16 + r) * 128] = dv[d][r];
     }
     __syncthreads();
-    if (half_of == 1) return;
+    if (half_of == 0) {
 #pragma unroll
-    for (int p = 0; p < MAPS; ++p)
+      for (int p = 0; p < MAPS; ++p)
 #pragma unroll
-      for (int d = 0; d < DQ / 32; ++d)
+        for (int d = 0; d < DQ / 32; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) dk[p][d][r] += y[((p * (DQ / 32) + d) * 16 + r) * 128];
+          for (int r = 0; r < 16; ++r) dk[p][d][r] += y[((p * (DQ / 32) + d) * 16 + r) * 128];
 #pragma unroll
-    for (int d = 0; d < DV / 32; ++d)
+      for (int d = 0; d < DV / 32; ++d)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) dv[d][r] += y[((MAPS * (DQ / 32) + d) * 16 + r) * 128];
-  }
-  if (!ok) return;
-  T* ko = (T*)a.dk + b * a.sdk[0] + key * a.sdk[1] + hk * a.sdk[2];
-  T* vo = (T*)a.dv + b * a.sdv[0] + key * a.sdv[1] + hk * a.sdv[2];
-  const float f = a.scale / rs;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-#pragma unroll
-    for (int p = 0; p < MAPS; ++p)
-#pragma unroll
-      for (int d = 0; d < DQ / 32; ++d) {
-        const int col = 32 * d + 8 * c + 4 * half;
-        f32x4 y = {dk[p][d][4 * c] * f, dk[p][d][4 * c + 1] * f, dk[p][d][4 * c + 2] * f, dk[p][d][4 * c + 3] * f};
-        if (col < a.D) El<TY>::store4(ko + (MAPS == 2 ? p * a.sdk[3] : 0) + col, y);
-      }
-#pragma unroll
-    for (int d = 0; d < DV / 32; ++d) {
-      const int col = 32 * d + 8 * c + 4 * half;
-      f32x4 y = {dv[d][4 * c], dv[d][4 * c + 1], dv[d][4 * c + 2], dv[d][4 * c + 3]};
-      if (col < a.Dv) El<TY>::store4(vo + col, y);
+        for (int r = 0; r < 16; ++r) dv[d][r] += y[((MAPS * (DQ / 32) + d) * 16 + r) * 128];
     }
+    __syncthreads();                                                 // past the join's reads
+    if (half_of == 1) return;
   }
+  if (key0 >= nk) return;
+  T* ko = (T*)a.dk + b * a.sdk[0] + key0 * a.sdk[1] + hk * a.sdk[2];
+  T* vo = (T*)a.dv + b * a.sdv[0] + key0 * a.sdv[1] + hk * a.sdv[2];
+  typedef RowStore<TY, DQ> OutK;
+  typedef RowStore<TY, DV> OutV;
+  char* piece = smem + wave * (OutK::BYTES > OutV::BYTES ? OutK::BYTES : OutV::BYTES);
+#pragma unroll
+  for (int p = 0; p < MAPS; ++p) OutK::store(dk[p], a.scale / rs, piece, ko + (MAPS == 2 ? p * a.sdk[3] : 0), a.sdk[1], nk - key0, a.D, lane);
+  OutV::store(dv, 1.0f, piece, vo, a.sdv[1], nk - key0, a.Dv, lane);
 }
 
 // A work-group a head and bucket: sums over samples and query blocks, in a fixed order.
@@ -661,10 +652,7 @@ __global__ __launch_bounds__(256) void diff_dw_kernel(AttnArgs a) {
 
 static inline int at_least(int a, int b) { return a > b ? a : b; }
 template <int TY, int MAPS, int DQ, int DV, bool BIAS, int RW> static int launch_dq(const AttnArgs* a, const BwdWork& wk, hipStream_t stream) {
-  constexpr int KT = TY == TY_F32 && RW == 4 ? 32 : 64, STAGE = 2 * KT * (MAPS * DQ + DV) * (int)sizeof(typename El<TY>::T);
-  constexpr int JOIN = RW == 2 ? (MAPS * DQ / 2 + 2) * 128 * 4 : 0;
-  static_assert(JOIN <= STAGE, "the halves' sums lie over the tiles");
-  const int lds = STAGE + (BIAS ? (5 * wk.nrel + 4 * DIAG) * 4 : 0);
+  const int lds = DqLds<TY, MAPS, DQ, DV, RW>::ALL + (BIAS ? (5 * wk.nrel + 4 * DIAG) * 4 : 0);
   if (int e = allow_lds<attn_dq_kernel<TY, MAPS, DQ, DV, BIAS, RW>>(lds)) return e;
   hipLaunchKernelGGL((attn_dq_kernel<TY, MAPS, DQ, DV, BIAS, RW>), dim3(a->B * a->H * wk.nblk), dim3(256), lds, stream, *a);
   SGTA_LAUNCH_CHECK();
@@ -673,7 +661,7 @@ template <int TY, int MAPS, int DQ, int DV, bool BIAS, int RW> static int launch
 template <int TY, int MAPS, int DQ, int DV, bool BIAS, int RW> static int launch_dkv(const AttnArgs* a, const BwdWork& wk, hipStream_t stream) {
   constexpr int STAGE = 2 * (64 * (MAPS * DQ + DV) * (int)sizeof(typename El<TY>::T) + 4 * MAPS * 64 * 4);
   constexpr int JOIN = RW == 2 ? (MAPS * DQ + DV) / 2 * 128 * 4 : 0;
-  const int nblk = cdiv(a->Lk, 32 * RW), lds = at_least(STAGE + (BIAS ? wk.nrel * 4 : 0), JOIN);
+  const int nblk = cdiv(a->Lk, 32 * RW), lds = at_least(STAGE + (BIAS ? wk.nrel * 4 : 0), at_least(JOIN, 4 * at_least(RowStore<TY, DQ>::BYTES, RowStore<TY, DV>::BYTES)));
   if (int e = allow_lds<attn_dkv_kernel<TY, MAPS, DQ, DV, BIAS, RW>>(lds)) return e;
   hipLaunchKernelGGL((attn_dkv_kernel<TY, MAPS, DQ, DV, BIAS, RW>), dim3(a->B * a->Hkv * nblk), dim3(256), lds, stream, *a, nblk);
   SGTA_LAUNCH_CHECK();

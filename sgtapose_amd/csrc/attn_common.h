@@ -219,6 +219,33 @@ __device__ __forceinline__ f32x16 zero16() {
   return z;
 }
 
+// A wave's 32 x COLS result, row li on lane li, to 32 rows of a strided matrix (those below ``rows``, elements below ``cols``): through
+// a piece of LDS of the wave's own, so that a store instruction writes whole runs of a row.  Straight from the registers it would
+// write 16 bytes to each of 32 rows.
+template <int TY, int COLS> struct RowStore {
+  typedef typename El<TY>::T T;
+  static constexpr int SZ = sizeof(T), PITCH = COLS * SZ + 16, BYTES = 32 * PITCH, PER = COLS * SZ / 16;
+  static __device__ __forceinline__ void store(const f32x16 (&v)[COLS / 32], float f, char* lds, T* out, long ld, int rows, int cols, int lane) {
+    const int li = lane & 31, half = lane >> 5;
+    asm volatile("" ::: "memory");                   // a wave's LDS operations are done in order; the compiler keeps it
+#pragma unroll
+    for (int d = 0; d < COLS / 32; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 x = {v[d][4 * g] * f, v[d][4 * g + 1] * f, v[d][4 * g + 2] * f, v[d][4 * g + 3] * f};
+        El<TY>::store4((T*)(lds + li * PITCH) + 32 * d + 8 * g + 4 * half, x);
+      }
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int p = 0; p < 32 * PER / 64; ++p) {
+      const int row = (p * 64 + lane) / PER, c = (p * 64 + lane) % PER * (16 / SZ);
+      const u32x4 x = *reinterpret_cast<const u32x4*>(lds + row * PITCH + c * SZ);
+      if (row < rows && c < cols) *reinterpret_cast<u32x4*>(out + row * ld + c) = x;
+    }
+    asm volatile("" ::: "memory");
+  }
+};
+
 // eight consecutive elements of a global row as an operand fragment (zero where ``ok`` is false)
 template <int TY> __device__ __forceinline__ typename El<TY>::Raw global_raw(const typename El<TY>::T* p, bool ok) {
   typename El<TY>::Raw f;

@@ -176,7 +176,7 @@ __global__ __launch_bounds__(256, TY == TY_F32 && MAPS * DQ + DV > 128 ? 1 : 2) 
   constexpr int KT = KeyTile<TY, RW>::KT, NK = RW == 2 || TY == TY_F32 || (MAPS == 2 && DV > 64) ? 32 : 64;   // keys at a time
   constexpr int MB = KT * DQ * (int)sizeof(T), KB = MAPS * MB, VB = KT * DV * (int)sizeof(T);
   extern __shared__ __align__(16) char smem[];       // 2 x (K maps, V), then the bias table
-  float* tab = reinterpret_cast<float*>(smem + 2 * (KB + VB));
+  float* tab = reinterpret_cast<float*>(smem + 2 * (KB + VB));       // nothing reads it when the epilogue lies over it
   const FwdPlace w = fwd_place(a, nblk);
   if (!w.ok) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, half = lane >> 5;
@@ -250,7 +250,7 @@ __global__ __launch_bounds__(256, TY == TY_F32 && MAPS * DQ + DV > 128 ? 1 : 2) 
       }
     }
     __syncthreads();
-    if (part == 1) return;
+    if (part == 0)
 #pragma unroll
     for (int p = 0; p < MAPS; ++p) {
       const float* y = x + p * (DV / 2 + 2) * 128;
@@ -274,35 +274,31 @@ __global__ __launch_bounds__(256, TY == TY_F32 && MAPS * DQ + DV > 128 ? 1 : 2) 
   for (int p = 0; p < MAPS; ++p) {
     const float l = half_sum(wv.l[p]);
     inv[p] = l == 0.0f ? 0.0f : 1.0f / l;
-    if (a.stats && row < nq && half == 0) {
+    if (a.stats && row < nq && half == 0 && part == 0) {
       // log2 of the sum beside its reference; a row that sees nothing gets weights of zero in the backward pass
       float* s = a.stats + 2 * ((((long)p * a.B + b) * a.H + h) * a.Lq + row);
       s[0] = l == 0.0f ? 0.0f : wv.m[p];
       s[1] = l == 0.0f ? INFINITY : log2f(l);
     }
   }
-  if (row < nq) {
-    T* op = (T*)a.out + b * a.so[0] + row * a.so[1] + h * a.so[2];
-    T* o2 = (MAPS == 2 && a.out2) ? (T*)a.out2 + (((long)b * a.Lq + row) * a.H + h) * a.Dv : nullptr;
-#pragma unroll
-    for (int d = 0; d < DV / 32; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int col = 32 * d + 8 * g + 4 * half;
-        if (col >= a.Dv) continue;
-        f32x4 x, y;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          x[r] = wv.o[0][d][4 * g + r] * inv[0];
-          if constexpr (MAPS == 2) {
-            y[r] = wv.o[1][d][4 * g + r] * inv[1];
-            x[r] = fmaf(-lam, y[r], x[r]);
-          }
-        }
-        El<TY>::store4(op + col, x);
-        if (MAPS == 2 && o2) El<TY>::store4(o2 + col, y);
-      }
+  typedef RowStore<TY, DV> Out;
+  char* piece = smem + wave * Out::BYTES;
+  if constexpr (RW == 2) {
+    __syncthreads();                                                 // past the join's reads
+    if (part == 1) return;
   }
+#pragma unroll
+  for (int d = 0; d < DV / 32; ++d) {
+    wv.o[0][d] *= inv[0];
+    if constexpr (MAPS == 2) {
+      wv.o[1][d] *= inv[1];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) wv.o[0][d][r] = fmaf(-lam, wv.o[1][d][r], wv.o[0][d][r]);
+    }
+  }
+  Out::store(wv.o[0], 1.0f, piece, (T*)a.out + b * a.so[0] + row0 * a.so[1] + h * a.so[2], a.so[1], nq - row0, a.Dv, lane);
+  if constexpr (MAPS == 2)
+    if (a.out2) Out::store(wv.o[1], 1.0f, piece, (T*)a.out2 + (((long)b * a.Lq + row0) * a.H + h) * a.Dv, (long)a.H * a.Dv, nq - row0, a.Dv, lane);
 }
 
 // ---- few queries ---------------------------------------------------------------------------------
@@ -579,7 +575,8 @@ template <typename L> static int step_resident(const AttnArgs* a, int tab) {
 
 template <int TY, int MAPS, int DQ, int DV, bool BIAS, int RW> static int launch_rows(const AttnArgs* a, int tab, hipStream_t stream) {
   constexpr int STAGE = 2 * KeyTile<TY, RW>::KT * (MAPS * DQ + DV) * (int)sizeof(typename El<TY>::T), JOIN = MAPS * (DV / 2 + 2) * 128 * 4;
-  const int lds = (RW == 2 && JOIN > STAGE ? JOIN : STAGE) + tab, nblk = cdiv(a->Lq, 32 * RW);
+  constexpr int OUT = 4 * RowStore<TY, DV>::BYTES, A = RW == 2 && JOIN > STAGE ? JOIN : STAGE;
+  const int lds = (OUT > A ? OUT : A) + tab, nblk = cdiv(a->Lq, 32 * RW);
   if (int e = allow_lds<attn_fwd_kernel<TY, MAPS, DQ, DV, BIAS, RW>>(lds)) return e;
   hipLaunchKernelGGL((attn_fwd_kernel<TY, MAPS, DQ, DV, BIAS, RW>), dim3(a->B * a->H * nblk), dim3(256), lds, stream, *a, nblk);
   SGTA_LAUNCH_CHECK();
