@@ -12,8 +12,9 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 // ---- quantisation of rows ------------------------------------------------------------------------
-// One work-group a row; up to 8192 elements stay in registers between the maximum and the quotients.  The quotient's rounding is
-// that of the exact quotient: the remainder x - q xs is exact in one fma for the q next to it, and decides.
+// A work-group a row; up to 8192 elements stay in registers between the maximum and the quotients.  The rounding is that of the
+// exact quotient: q = rint(x (1 / xs)) is at most one off, and the remainder x - q xs, exact in one fma for the q next to the
+// quotient, tells.  16384 x 4096 bfloat16: 201 MB in 42 us, the rate of a copy (a wave a row: 55 us).
 template <int TY> __device__ __forceinline__ void load8(const typename El<TY>::T* p, int k, int K, bool vec, float (&v)[8]) {
   if (vec && k + 8 <= K) {
     const typename El<TY>::Raw f = *reinterpret_cast<const typename El<TY>::Raw*>(p + k);
@@ -25,6 +26,7 @@ template <int TY> __device__ __forceinline__ void load8(const typename El<TY>::T
   }
 }
 
+// one quotient with every case: subnormal scales, rows of zeros, what is not finite
 __device__ __forceinline__ int quant1(float x, float s, float inv) {
   float q = rintf(x * inv);                            // inv overflows only where s is subnormal
   if (!(fabsf(q) <= 128.0f)) q = rintf(x / s);
@@ -34,26 +36,48 @@ __device__ __forceinline__ int quant1(float x, float s, float inv) {
   return (int)fminf(fmaxf(q, -127.0f), 127.0f);
 }
 
+// eight quotients as bytes
+__device__ __forceinline__ unsigned long long quant8(const float (&v)[8], float s, float inv) {
+  // 1.5 2^23 + x inv: the sum's rounding is rint, and its low byte is the quotient's
+  constexpr float BIG = 12582912.0f;
+  unsigned t[8];
+  const float h = 0.5f * s;
+  bool odd = !(s >= 1e-30f && s < INFINITY);           // scales whose half or inverse may not be exact
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float b = fmaf(v[e], inv, BIG), r = fmaf(-(b - BIG), s, v[e]);
+    odd |= !(fabsf(r) < h);
+    t[e] = __float_as_uint(b);
+  }
+  if (odd) {                                           // a quotient at a half or on the other side of one: rare
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] = (unsigned)quant1(v[e], s, inv);
+  }
+  const unsigned lo = __builtin_amdgcn_perm(t[1], t[0], 0x0c0c0400u) | __builtin_amdgcn_perm(t[3], t[2], 0x04000c0cu);
+  const unsigned hi = __builtin_amdgcn_perm(t[5], t[4], 0x0c0c0400u) | __builtin_amdgcn_perm(t[7], t[6], 0x04000c0cu);
+  return (unsigned long long)hi << 32 | lo;
+}
+
 template <int TY>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const void* xv, long ldx, signed char* xq, long ldq, float* xs, int K) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const long m = blockIdx.x;
   const typename El<TY>::T* x = (const typename El<TY>::T*)xv + m * ldx;
   signed char* o = xq + m * ldq;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const bool vec = (uintptr_t)x % 16 == 0, vec8 = (uintptr_t)o % 8 == 0;
-  constexpr int KEEP = 4;
+  constexpr int KEEP = 4, NT = 256;
   float v[KEEP][8];
   unsigned top = 0;                                    // |x| by its bits: a not-a-number is the largest
 #pragma unroll
   for (int i = 0; i < KEEP; ++i) {
-    const int k = (i * 256 + tid) * 8;
+    const int k = (i * NT + tid) * 8;
     if (k < K) {
       load8<TY>(x, k, K, vec, v[i]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[i][e]) & 0x7fffffffu);
     }
   }
-  for (int k = (KEEP * 256 + tid) * 8; k < K; k += 2048) {
+  for (int k = (KEEP * NT + tid) * 8; k < K; k += NT * 8) {
     float t[8];
     load8<TY>(x, k, K, vec, t);
 #pragma unroll
@@ -69,8 +93,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const void* xv, long ld
   if (tid == 0) xs[m] = s;
   auto write = [&](int k, const float (&t)[8]) {
     union { signed char c[8]; unsigned long long u; } b;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) b.c[e] = (signed char)quant1(t[e], s, inv);
+    b.u = quant8(t, s, inv);
     if (vec8 && k + 8 <= K) {
       *reinterpret_cast<unsigned long long*>(o + k) = b.u;
     } else {
@@ -81,10 +104,10 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const void* xv, long ld
   };
 #pragma unroll
   for (int i = 0; i < KEEP; ++i) {
-    const int k = (i * 256 + tid) * 8;
+    const int k = (i * NT + tid) * 8;
     if (k < K) write(k, v[i]);
   }
-  for (int k = (KEEP * 256 + tid) * 8; k < K; k += 2048) {
+  for (int k = (KEEP * NT + tid) * 8; k < K; k += NT * 8) {
     float t[8];
     load8<TY>(x, k, K, vec, t);
     write(k, t);

@@ -31,7 +31,7 @@ def _rows(name, shape, stride, dtype, dtypes, want=None):
 
 
 def _vector(name, t, n, dtype):
-    if t.shape != (n,) or t.dtype != dtype or (n > 1 and t.stride(0) != 1):
+    if t.shape != (n,) or t.dtype != dtype or not t.is_contiguous():
         _fail("%s: %s %s where %s [%d] is expected", name, t.dtype, tuple(t.shape), dtype, n)
 
 

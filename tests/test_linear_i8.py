@@ -88,7 +88,7 @@ def test_longest_sum_is_exact():
 @gpu
 @pytest.mark.parametrize("dtype", ALL, ids=IDS.get)
 def test_quantize_rows(dtype):
-    for M, K in ((1, 1), (3, 7), (5, 64), (130, 343), (4, 4096), (3, 8200), (2, 20001)):
+    for M, K in ((1, 1), (3, 7), (5, 64), (130, 343), (4, 4096), (3, 8200), (2, 20001), (4097, 40), (4100, 4105)):
         g = torch.Generator().manual_seed(K)
         x = (torch.randn(M, K, generator=g) * torch.exp(torch.randn(M, 1, generator=g) * 4)).to(dtype)
         if M > 2:
