@@ -46,12 +46,14 @@ struct BwdWork {
 // LDS of attn_dq_kernel before the bias table: two stages of keys, or what lies over them at the end
 template <int TY, int MAPS, int DQ, int DV, int RW> struct DqLds {
   static constexpr int KT = TY == TY_F32 && RW == 4 ? 32 : 64, STAGE = 2 * KT * (MAPS * DQ + DV) * (int)sizeof(typename El<TY>::T);
-  static constexpr int JOIN = RW == 2 ? (MAPS * DQ / 2 + 2) * 128 * 4 : 0, OUT = 4 * RowStore<TY, DQ>::BYTES;
+  static constexpr int JOIN = RW == 2 ? MAPS * (DQ / 2 + 2) * 128 * 4 : 0, OUT = 4 * RowStore<TY, DQ>::BYTES;
   static constexpr int ALL = OUT > STAGE ? OUT : STAGE;
   static_assert(JOIN <= STAGE, "the halves' sums lie over the tiles");
 };
+// float heads of 32 keep three work-groups on a CU at the price of a few registers stored outside the loop: 52 us where two take 67
+// (136 windows of 144 tokens).
 template <int TY, int MAPS, int DQ, int DV, bool BIAS, int RW>
-__global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2) void attn_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : DQ + DV > 64 || MAPS > 1 ? 2 : 3) void attn_dq_kernel(AttnArgs a) {
   typedef typename El<TY>::T T;
   typedef typename El<TY>::Frag Frag;
   constexpr int KT = DqLds<TY, MAPS, DQ, DV, RW>::KT;
@@ -145,7 +147,6 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
       const long at = (((long)p * a.B + b) * a.H + h) * a.Lq + row;
       m[p] = ok ? a.stats[2 * at] : 0.0f;
       lg[p] = ok ? a.stats[2 * at + 1] : INFINITY;
-      if (ok && half == 0) a.ws[wk.delta + at] = dl[p];
     }
     float t = top;
 #pragma unroll
@@ -153,13 +154,6 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
     if (lane == 0) red[wave] = t;
     __syncthreads();
     if (tid == 0) *topw = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    if constexpr (MAPS == 2) {
-      __syncthreads();
-      const float t2 = wave_sum(half == 0 && half_of == 0 && ok ? dl[1] : 0.0f);
-      if (lane == 0) red[wave] = t2;
-      __syncthreads();
-      if (tid == 0) part[0] = (red[0] + red[1]) + (red[2] + red[3]);
-    }
   }
   const float rs = TY == TY_F16 ? pow2_to_one(top) : 1.0f;          // power of two for dS
   const float irs = 1.0f / rs;
@@ -167,7 +161,9 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
   const int pos = st + row, pmin = st + row0, pmax = st + row0 + 31;
   const int limit = min(nk - 1, a.causal ? pos : nk - 1), low = min(nk - 1, a.causal ? pmin : nk - 1);
   // by row: sums of dS over all keys; of dS and P over the keys left and right of ``reach``
-  float far_l = 0.0f, far_r = 0.0f, sum_l = 0.0f, sum_r = 0.0f, sum_n = 0.0f, p_l = 0.0f, p_r = 0.0f;
+  float far_l = 0.0f, far_r = 0.0f, sum_l = 0.0f, sum_r = 0.0f, p_l = 0.0f, p_r = 0.0f;
+  // sums of P (X - delta) by map, which are zero but for delta's error: it comes from outputs whose weights and values were rounded
+  float err[MAPS] = {};
   bool fold = true;
   const float* tb = tab;
   float *hist = nullptr, *diag = nullptr;
@@ -204,10 +200,11 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
       const bool masked = low < j0 + 31;
       const bool left = BIAS && j0 + 31 - pmin <= -a.reach, right = BIAS && j0 - pmax >= a.reach;
       const bool plain = !masked && (!BIAS || (fold && (left || right)));
-      f32x16 x = zero16();
+      Products<TY, true> xsum(zero16());
 #pragma unroll
       for (int k = 0; k < DV / 16; ++k)
-        if (DV > 32 || k == 0 || both) x = El<TY>::mma(TV::read_rows(vt, 32 * u + li, k, half), g[k], x);
+        if (DV > 32 || k == 0 || both) xsum.add(TV::read_rows(vt, 32 * u + li, k, half), g[k]);
+      const f32x16 x = xsum.get();
       Frag df[MAPS][2];
 #pragma unroll
       for (int p = 0; p < MAPS; ++p) {
@@ -243,14 +240,14 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
         for (int r = 0; r < 16; ++r) {
           const float d = s[r] * (TY == TY_F16 ? fmaf(x[r], rs, -dl[p] * rs) : x[r] - dl[p]);
           s[r] = (MAPS == 2 && p == 1) ? d * sg : d;
-          if (BIAS) tot[r & 1] += s[r];
+          tot[r & 1] += d;
         }
+        const float all = (tot[0] + tot[1]) * irs;
+        err[p] += all;
         if constexpr (BIAS) {
-          const float all = (tot[0] + tot[1]) * irs;
           if (left) sum_l += all;
           else if (right) sum_r += all;
           else {
-            sum_n += all;
             // Sums by distance, 16 keys at a time: the tile as rows of 32 with 15 zeros between them (row k at 47 k, the zeros stay),
             // where the entries of one distance, k - q, lie 48 apart; lane u < 47 adds up those of distance 15 - u.  (LDS atomics
             // into the sums take two cycles a lane: 16 of them cost 1950 cycles a tile.)
@@ -289,11 +286,12 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
     __syncthreads();
   }
 
-  float e = half_sum((sum_l + sum_r) + sum_n);                       // of a row's dS over all its keys
+#pragma unroll
+  for (int p = 0; p < MAPS; ++p) err[p] = half_sum(err[p]);
   if constexpr (RW == 2) {
     // the second half's sums, register by register, over the tiles: every wave is past its last read
     float* y = reinterpret_cast<float*>(smem) + (wave & 1) * 64 + lane;
-    float* z = reinterpret_cast<float*>(smem) + MAPS * DQ / 2 * 128 + (wave & 1) * 128 + half_of * 64 + lane;
+    float* z = reinterpret_cast<float*>(smem) + MAPS * DQ / 2 * 128 + (wave & 1) * (MAPS * 128) + half_of * 64 + lane;
     if (half_of == 1) {
 #pragma unroll
       for (int p = 0; p < MAPS; ++p)
@@ -302,7 +300,8 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
 #pragma unroll
           for (int r = 0; r < 16; ++r) y[((p * (DQ / 32) + d) * 16 + r) * 128] = dq[p][d][r];
     }
-    if (BIAS) z[0] = e;
+#pragma unroll
+    for (int p = 0; p < MAPS; ++p) z[p * 128] = err[p];
     __syncthreads();
     if (half_of == 0) {
 #pragma unroll
@@ -312,7 +311,8 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
 #pragma unroll
           for (int r = 0; r < 16; ++r) dq[p][d][r] += y[((p * (DQ / 32) + d) * 16 + r) * 128];
     }
-    if (BIAS) e += z[half_of ? -64 : 64];
+#pragma unroll
+    for (int p = 0; p < MAPS; ++p) err[p] += z[p * 128 + (half_of ? -64 : 64)];
   }
   typedef RowStore<TY, DQ> Out;
   if (RW == 2) __syncthreads();                                      // past the join's reads
@@ -321,11 +321,24 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : 2
 #pragma unroll
     for (int p = 0; p < MAPS; ++p) Out::store(dq[p], a.scale * irs, smem + wave * Out::BYTES, o + (MAPS == 2 ? p * a.sdq[3] : 0), a.sdq[1], nq - row0, a.D, lane);
   }
+  // The kernel of dK and dV and the gradient of lambda get delta without its error (bfloat16, 2048 tokens: dK is 2.5e-3 off with it,
+  // 2.36e-3 without, of which 1.66e-3 is dK's own rounding; lambda's 4.4e-3 and 1.2e-3).
+#pragma unroll
+  for (int p = 0; p < MAPS; ++p) {
+    dl[p] += err[p];
+    if (ok && half == 0 && half_of == 0) a.ws[wk.delta + (((long)p * a.B + b) * a.H + h) * a.Lq + row] = dl[p];
+  }
+  if constexpr (MAPS == 2) {
+    const float t2 = wave_sum(half == 0 && half_of == 0 && ok ? dl[1] : 0.0f);
+    __syncthreads();
+    if (lane == 0) red[wave] = t2;
+    __syncthreads();
+    if (tid == 0) part[0] = (red[0] + red[1]) + (red[2] + red[3]);
+  }
   if constexpr (BIAS) {
-    // A row's dS sums to zero, but for delta's error (it comes from an output that was rounded): of the far buckets, where P's
-    // sum is large, that error times the sum is taken off again.
-    sum_l = wave_sum(ok ? fmaf(-e, p_l, sum_l) : 0.0f);
-    sum_r = wave_sum(ok ? fmaf(-e, p_r, sum_r) : 0.0f);
+    // off the far buckets, where P's sum is large, comes the error times that sum
+    sum_l = wave_sum(ok ? fmaf(-err[0], p_l, sum_l) : 0.0f);
+    sum_r = wave_sum(ok ? fmaf(-err[0], p_r, sum_r) : 0.0f);
     if (lane == 0) {                                  // the ends of the table stand for everything beyond
       tab[(1 + wave) * wk.nrel] += sum_l;
       tab[(2 + wave) * wk.nrel - 1] += sum_r;
@@ -488,19 +501,20 @@ __global__ __launch_bounds__(256, (MAPS * DQ + DV > 128 || (TY == TY_F32 && MAPS
         }
         return v;
       };
-      f32x16 x = rows16(0, 1);                                       // X - delta: the product starts from -delta
+      Products<TY> xsum(rows16(0, 1));                               // X - delta: the sum starts from -delta
 #pragma unroll
       for (int k = 0; k < DV / 16; ++k)
-        if (DV > 32 || k == 0 || both) x = El<TY>::mma(TG::read_rows(gt, 32 * u + li, k, half), vf[k], x);
-      f32x16 w0;
+        if (DV > 32 || k == 0 || both) xsum.add(TG::read_rows(gt, 32 * u + li, k, half), vf[k]);
+      f32x16 x = xsum.get(), w0;
       Frag dsf[MAPS][2];
 #pragma unroll
       for (int p = 0; p < MAPS; ++p) {
-        f32x16 s = zero16();
-        if (plain) s = rows16(p, 0);                                 // and the exponent from (-m - lg) / c2
+        // and the exponent from (-m - lg) / c2
+        Products<TY> ssum(plain ? rows16(p, 0) : zero16());
 #pragma unroll
         for (int k = 0; k < DQ / 16; ++k)
-          if (DQ > 32 || k == 0 || both) s = El<TY>::mma(TQ::read_rows(qt + p * MB, 32 * u + li, k, half), kf[p][k], s);
+          if (DQ > 32 || k == 0 || both) ssum.add(TQ::read_rows(qt + p * MB, 32 * u + li, k, half), kf[p][k]);
+        f32x16 s = ssum.get();
         if (plain) {
           const float far = !BIAS ? 0.0f : left ? far_l : far_r;
 #pragma unroll

@@ -59,14 +59,17 @@ template <> struct El<TY_F32> {
   typedef float T;
   typedef Split8 Frag;         // an operand fragment
   typedef f32x8 Raw;           // eight elements as they lie in memory
-  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+  static __device__ __forceinline__ f32x16 mma_small(Frag a, Frag b, f32x16 c) {
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.lo, b.hi, c, 0, 0, 0);
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.hi, b.lo, c, 0, 0, 0);
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.mid, b.mid, c, 0, 0, 0);
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.mid, b.hi, c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.hi, b.mid, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.hi, b.mid, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16 mma_large(Frag a, Frag b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.hi, b.hi, c, 0, 0, 0);
   }
+  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) { return mma_large(a, b, mma_small(a, b, c)); }
   static __device__ __forceinline__ Frag frag(f32x8 v) { return split8(v); }
   static __device__ __forceinline__ Frag frag_of(Raw v) { return split8(v); }
   static __device__ __forceinline__ float load(const T* p) { return *p; }
@@ -218,6 +221,31 @@ __device__ __forceinline__ f32x16 zero16() {
   const f32x16 z = {0};
   return z;
 }
+
+// The sum of a few products from ``start`` on.  float: the matrix pipe cuts off what lies below its largest term towards minus
+// infinity.  A start far larger than the products (an exponent's maximum) would cost them bits, so the vector pipe adds it at the end
+// (777 tokens: dK and dV 1.3e-6 off from such a start, 6e-7 so).  With APART the products of the upper parts, which lose nothing to
+// speak of, have an accumulator of their own beside the small ones: the mean error of an instruction, -3e-8, otherwise adds up over the
+// thousands of pairs of a bias table's bucket (its gradient 1.8e-6 off, and 3.5e-7 so).
+template <int TY, bool APART = false> struct Products {
+  f32x16 sum;
+  __device__ __forceinline__ Products(f32x16 start) : sum(start) {}
+  __device__ __forceinline__ void add(typename El<TY>::Frag a, typename El<TY>::Frag b) { sum = El<TY>::mma(a, b, sum); }
+  __device__ __forceinline__ f32x16 get() const { return sum; }
+};
+template <bool APART> struct Products<TY_F32, APART> {
+  f32x16 start, sum, rest;
+  __device__ __forceinline__ Products(f32x16 start) : start(start), sum(zero16()), rest(zero16()) {}
+  __device__ __forceinline__ void add(Split8 a, Split8 b) {
+    if (APART) {
+      rest = El<TY_F32>::mma_small(a, b, rest);
+      sum = El<TY_F32>::mma_large(a, b, sum);
+    } else {
+      sum = El<TY_F32>::mma(a, b, sum);
+    }
+  }
+  __device__ __forceinline__ f32x16 get() const { return (APART ? sum + rest : sum) + start; }
+};
 
 // A wave's 32 x COLS result, row li on lane li, to 32 rows of a strided matrix (those below ``rows``, elements below ``cols``): through
 // a piece of LDS of the wave's own, so that a store instruction writes whole runs of a row.  Straight from the registers it would
