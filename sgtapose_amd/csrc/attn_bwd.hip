@@ -31,7 +31,8 @@ struct BwdWork {
   long total;
   int rw, nblk, nsum, nrel;    // attn_dq_kernel's waves by rows and query blocks; floats of a part; distances told apart
   __host__ __device__ BwdWork(const AttnArgs& a, int maps) {
-    rw = row_waves((long)a.B * a.H * ((a.Lq + 127) / 128));
+    // (float heads beyond 64: the tiles of two halves leave no room for four waves' sums by distance of a wide table)
+    rw = maps == 1 && a.dtype == TY_F32 && a.D > 64 && a.reach > 256 ? 4 : row_waves((long)a.B * a.H * ((a.Lq + 127) / 128));
     nblk = (a.Lq + 32 * rw - 1) / (32 * rw);
     nrel = 2 * (a.reach + BIAS_PAD) + 1;
     nsum = maps == 1 ? a.num_buckets : 1;
@@ -695,7 +696,7 @@ template <int TY, int MAPS, int DQ, int DV, bool BIAS> static int launch_bwd(con
 static int bwd_check(const AttnArgs* a, int maps) {
   if (int e = attn_check(a, maps)) return e;
   if (!a->dout || !a->dq || !a->dk || !a->dv || !a->dw || !a->stats || !a->ws || (maps == 2 && !a->out2)) return SGTA_EBADARG;
-  if (a->ws_floats < BwdWork(*a, maps).total) return SGTA_EBADARG;
+  if (a->ws_floats < BwdWork(*a, maps).total || (uintptr_t)a->ws % 16) return SGTA_EBADARG;
   const int al = a->dtype == TY_F32 ? 4 : 8;
   const long* s[] = {a->sdo, a->sdq, a->sdk, a->sdv};
   const void* p[] = {a->dout, a->dq, a->dk, a->dv};

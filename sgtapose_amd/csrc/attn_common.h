@@ -214,6 +214,7 @@ template <int TY, int COLS, int ROWS, int NT> struct Dma {
 // forward 93 -> 76, dK dV 122 -> 93, dQ 85 -> 60; 768 (32 x 8 heads, 343) 36 -> 39, 65 -> 71, 52 -> 76.
 __host__ __device__ __forceinline__ int row_waves(long groups) { return groups < 704 ? 2 : 4; }
 #define MAX_PITCH (1 << 24)
+#define MAX_GROUPS (1L << 24)  // work-groups of 256 in a launch: a grid's work-items are counted in 32 bits
 // until at most KEEP of this wave's loads are in flight
 template <int KEEP> __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(KEEP) : "memory"); }
 

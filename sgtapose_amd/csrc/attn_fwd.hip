@@ -589,7 +589,7 @@ static int launch_fwd(const AttnArgs* a, hipStream_t stream) {
     typedef StepTile<TY, MAPS, DQ, DV> L;
     const int splits = step_splits(a, step_resident<L>(a, tab)), G = a->H / a->Hkv;
     const long rows = (long)a->B * a->Hkv * MAPS * a->Lq * G;
-    if (splits > 1 && (!a->ws || a->ws_floats < splits * rows * (DV + 4))) return SGTA_EBADARG;
+    if (splits > 1 && (!a->ws || (uintptr_t)a->ws % 16 || a->ws_floats < splits * rows * (DV + 4))) return SGTA_EBADARG;
     const int lds = step_lds<L>(a, tab);
     if (int e = allow_lds<attn_step_kernel<TY, MAPS, DQ, DV, BIAS>>(lds)) return e;
     hipLaunchKernelGGL((attn_step_kernel<TY, MAPS, DQ, DV, BIAS>), dim3(a->B * a->Hkv * splits), dim3(256), lds, stream, *a, splits);
@@ -611,13 +611,14 @@ int attn_check(const AttnArgs* a, int maps) {
   if (a->dtype < 0 || a->dtype > 2 || a->B < 1 || a->Lq < 1 || a->Lk < 1 || a->H < 1 || a->Hkv < 1 || a->H % a->Hkv) return SGTA_EBADARG;
   if (a->D < 8 || a->D % 8 || a->Dv < 8 || a->Dv % 8 || !(a->scale > 0.0f) || !(a->scale < INFINITY)) return SGTA_EBADARG;
   if (maps == 1 ? (a->D > 128 || a->Dv != a->D) : (a->D > 64 || a->Dv > 128)) return SGTA_EBADARG;
-  if (a->Lq >= 1 << 29 || a->Lk >= 1 << 29 || (long)a->B * a->H * cdiv(a->Lq > a->Lk ? a->Lq : a->Lk, 32) >= 1L << 31) return SGTA_ETOOBIG;
+  if (a->Lq >= 1 << 29 || a->Lk >= 1 << 29 || (long)a->B * a->H * cdiv(a->Lq > a->Lk ? a->Lq : a->Lk, 128) >= MAX_GROUPS) return SGTA_ETOOBIG;
   if (maps == 1 && (!a->lut || a->reach < 1 || a->reach > 1024 || a->num_buckets < 1)) return SGTA_EBADARG;
   const int al = a->dtype == TY_F32 ? 4 : 8;           // strides and pointers: whole 16-byte pieces
   const long* s[] = {a->sq, a->sk, a->sv, a->so};
   const void* p[] = {a->q, a->k, a->v, a->out};
   for (int i = 0; i < 3; ++i)
     if (s[i][1] > MAX_PITCH / (a->dtype == TY_F32 ? 4 : 2) || s[i][1] < 0) return SGTA_ETOOBIG;
+  if (maps == 2 && (uintptr_t)a->out2 % 16) return SGTA_EBADARG;
   for (int i = 0; i < 4; ++i) {
     if ((uintptr_t)p[i] % 16) return SGTA_EBADARG;
     for (int j = 0; j < (i < 2 && maps == 2 ? 4 : 3); ++j)

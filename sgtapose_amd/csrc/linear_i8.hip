@@ -504,7 +504,7 @@ __global__ __launch_bounds__(1024) void linear_i8_few_kernel(I8Args a) {
 
 template <int BM, int BN, int WM, int WN, bool RAGGED> static int launch_i8(const I8Args& a, hipStream_t st) {
   const int tm = cdiv(a.M, BM), tn = cdiv(a.N, BN), lds = 2 * (BM + BN) * 128;
-  if ((long)tm * tn > 0x7ffffff0L) return SGTA_ETOOBIG;
+  if ((long)tm * tn >= MAX_GROUPS - 8) return SGTA_ETOOBIG;
   if (int e = allow_lds<linear_i8_kernel<BM, BN, WM, WN, RAGGED>>(lds)) return e;
   hipLaunchKernelGGL((linear_i8_kernel<BM, BN, WM, WN, RAGGED>), dim3((tm * tn + 7) / 8 * 8), dim3(64 * WM * WN), lds, st, a, tm, tn);
   SGTA_LAUNCH_CHECK();
@@ -512,13 +512,14 @@ template <int BM, int BN, int WM, int WN, bool RAGGED> static int launch_i8(cons
 }
 static int launch_i8_large(const I8Args& a, hipStream_t st) {
   const int tm = cdiv(a.M, 256), tn = cdiv(a.N, 256), lds = 2 * 512 * 128;
-  if ((long)tm * tn > 0x7ffffff0L) return SGTA_ETOOBIG;
+  if ((long)tm * tn >= MAX_GROUPS - 8) return SGTA_ETOOBIG;
   if (int e = allow_lds<linear_i8_large_kernel>(lds)) return e;
   hipLaunchKernelGGL(linear_i8_large_kernel, dim3((tm * tn + 7) / 8 * 8), dim3(256), lds, st, a, tm, tn);
   SGTA_LAUNCH_CHECK();
   return SGTA_OK;
 }
 template <int MT, bool RAGGED> static int launch_few(const I8Args& a, hipStream_t st) {
+  if (cdiv(a.N, 16) >= MAX_GROUPS / 4) return SGTA_ETOOBIG;          // work-groups of 1024
   hipLaunchKernelGGL((linear_i8_few_kernel<MT, RAGGED>), dim3(cdiv(a.N, 16), cdiv(a.M, 16 * MT)), dim3(1024), 0, st, a);
   SGTA_LAUNCH_CHECK();
   return SGTA_OK;
@@ -527,10 +528,15 @@ template <int MT, bool RAGGED> static int launch_few(const I8Args& a, hipStream_
 extern "C" int sgta_quant_rows_i8(const void* x, long ldx, int dtype, signed char* xq, long ldq, float* xs, int M, int K, sgta_stream_t stream) {
   if (!x || !xq || !xs || M < 1 || K < 1 || ldx < K || ldq < K || dtype < 0 || dtype > 2) return SGTA_EBADARG;
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == TY_F32) hipLaunchKernelGGL(quant_rows_kernel<TY_F32>, dim3(M), dim3(256), 0, st, x, ldx, xq, ldq, xs, K);
-  else if (dtype == TY_F16) hipLaunchKernelGGL(quant_rows_kernel<TY_F16>, dim3(M), dim3(256), 0, st, x, ldx, xq, ldq, xs, K);
-  else hipLaunchKernelGGL(quant_rows_kernel<TY_BF16>, dim3(M), dim3(256), 0, st, x, ldx, xq, ldq, xs, K);
-  SGTA_LAUNCH_CHECK();
+  for (long m = 0; m < M; m += MAX_GROUPS / 2) {         // a launch each 2^23 rows
+    const dim3 rows(M - m < MAX_GROUPS / 2 ? M - m : MAX_GROUPS / 2);
+    const char* p = (const char*)x + m * ldx * (dtype == TY_F32 ? 4 : 2);
+    signed char* o = xq + m * ldq;
+    if (dtype == TY_F32) hipLaunchKernelGGL(quant_rows_kernel<TY_F32>, rows, dim3(256), 0, st, p, ldx, o, ldq, xs + m, K);
+    else if (dtype == TY_F16) hipLaunchKernelGGL(quant_rows_kernel<TY_F16>, rows, dim3(256), 0, st, p, ldx, o, ldq, xs + m, K);
+    else hipLaunchKernelGGL(quant_rows_kernel<TY_BF16>, rows, dim3(256), 0, st, p, ldx, o, ldq, xs + m, K);
+    SGTA_LAUNCH_CHECK();
+  }
   return SGTA_OK;
 }
 

@@ -13,8 +13,13 @@ Lengths: ``kv_len`` / ``q_len`` int32 [B] on the GPU (None: all).  What lies beh
 the first query among the keys (None: 0); a new token against a cache that already holds it has q_start = kv_len - 1.
 ``causal``: a query at position p sees keys j <= p.  A query that sees no key has an output and gradients of zero.
 
+Within the lengths a value that is not finite may also reach positions from which the mask hides it (0 times infinity), as in the
+plain products.  float32 operands are split into three bfloat16 numbers, so that an infinity among them gives not-a-numbers.
+
 Everything is enqueued on the current stream of the tensors' device; workspaces come from torch's allocator anew in each call, so
-calls on several streams and calls captured into several graphs do not share any.
+calls on several streams and calls captured into several graphs do not share any.  Outputs share no memory with each other or with
+what a call reads.  ``rel_attention`` puts the table of buckets on the device at its first call with given settings, which cannot be
+captured: run it once before a graph is.
 """
 import ctypes
 import functools
@@ -76,6 +81,9 @@ def relative_buckets(num_buckets, max_distance, bidirectional):
 def _lut(num_buckets, max_distance, bidirectional, device):
     """``relative_buckets`` on the device, and each bucket's first entry and number of entries: depends on nothing but the arguments,
     as ops.gauss_taps."""
+    if torch.cuda.is_current_stream_capturing():
+        _fail("the table of %d buckets to distance %d is not on the device yet and cannot be copied there in a captured graph: call the operator "
+              "once before", num_buckets, max_distance)
     of = relative_buckets(num_buckets, max_distance, bidirectional)
     count = [of.count(b) for b in range(num_buckets)]
     first = [of.index(b) if n else 0 for b, n in enumerate(count)]
@@ -270,7 +278,8 @@ def _backward(name, maps, a, like, dout, w, out, saved, grads, q_len, kv_len):
     shape = (a.B, a.Lq, a.H, a.Dv)
     _set_strides(a, "sdo", _like("dout", dout, shape, like), False)
     _set_strides(a, "so", _like("out", out, shape, like), False)
-    if tuple(stats.shape) != (maps, a.B, a.H, a.Lq, 2) or stats.device != like.device or (maps == 2 and tuple(out2.shape) != shape):
+    if tuple(stats.shape) != (maps, a.B, a.H, a.Lq, 2) or stats.device != like.device or (out2 is None) != (maps == 1) or (
+            maps == 2 and (tuple(out2.shape) != shape or out2.dtype != like.dtype)):
         _fail("saved does not come from a forward call of this shape")
     a.dout, a.out, a.stats = dout.data_ptr(), out.data_ptr(), stats.data_ptr()
     if maps == 2:

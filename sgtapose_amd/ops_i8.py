@@ -4,7 +4,7 @@
     wq, ws = quantize_rows(w)                       # weights [N, K], once
     out = linear_i8(xq, xs, wq, ws, bias, relu=..., dtype=torch.bfloat16)
 
-x, bias and out are float32, float16 or bfloat16; scales are float32; the sums are exact whole numbers.  Everything is enqueued on
+x, bias and out are float32, float16 or bfloat16; scales are float32; the sums are exact whole numbers.  Outputs share no memory with what a call reads.  Everything is enqueued on
 the current stream of the tensors' device.
 """
 import functools

@@ -591,3 +591,54 @@ def test_backward_refuses():
         a = _lib.AttnArgs(**{**ok, **change})
         assert lib.sgta_rel_attn_bwd(ctypes.byref(a), None) < 0, change
     assert lib.sgta_diff_attn_bwd(ctypes.byref(_lib.AttnArgs(**ok)), None) < 0      # no second map's product
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ALL, ids=NAMES.get)
+def test_widest_tables_and_heads(dtype):
+    """The largest tables with the largest heads: what a work-group keeps still fits it."""
+    for buckets, far in ((256, 1024), (64, 300)):
+        check_both(Case(1, dtype, 1, 150, 200, 2, 1, 128, buckets=buckets, far=far, seed=5))
+        check_both(Case(1, dtype, 1, 70, 180, 8, 1, 128, causal=True, buckets=buckets, far=far, q_start=[110], seed=6))
+        check_forward(Case(1, dtype, 1, 1, 700, 16, 1, 128, causal=True, buckets=buckets, far=far, q_start=[699], seed=7))
+
+
+@gpu
+def test_first_call_with_a_table_is_not_captured():
+    c = Case(1, torch.bfloat16, 1, 40, 50, 2, 2, 32, buckets=24, far=77)
+    t = [x.cuda() for x in (c.q, c.k, c.v, c.w)]
+    out = torch.empty_like(t[0])
+    with pytest.raises(SgtaHipError, match="captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            ops_attn.rel_attention(*t, out, **c.kwargs("cpu"))
+    want = ops_attn.rel_attention(*t, **c.kwargs("cpu"))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops_attn.rel_attention(*t, out, **c.kwargs("cpu"))
+    for _ in range(2):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+@gpu
+def test_saved_must_fit():
+    c = Case(2, torch.bfloat16, 1, 20, 30, 2, 2, 32)
+    t = [x.cuda() for x in (c.q, c.k, c.v, c.w)]
+    out, (stats, out2) = ops_attn.diff_attention(*t, save=True)
+    for saved in ((stats, None), (stats, out2.float()), (stats[:, :, :1], out2)):
+        with pytest.raises(SgtaHipError, match="saved"):
+            ops_attn.diff_attention_bwd(c.dout.cuda(), *t, out, saved)
+
+
+@gpu
+def test_positions_too_far_apart_are_refused():
+    """Two rows of a tensor of 2^24 + 16 bytes a position (an untouched allocation; nothing is launched)."""
+    wide = torch.empty(2, (1 << 23) + 8, dtype=torch.bfloat16, device="cuda")
+    far = wide[:, :64].view(1, 2, 2, 32)
+    near = torch.zeros(1, 2, 2, 32, dtype=torch.bfloat16, device="cuda")
+    table = torch.zeros(32, 2, dtype=torch.bfloat16, device="cuda")
+    for args in ((far, near, near), (near, far, near), (near, near, far)):
+        with pytest.raises(SgtaHipError, match="bytes apart"):
+            ops_attn.rel_attention(*args, table)

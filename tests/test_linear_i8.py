@@ -183,3 +183,16 @@ def test_c_entries_refuse_before_they_launch():
         a = list(ok)
         a[at] = v
         assert lib.sgta_quant_rows_i8(*a) < 0, (at, v)
+
+
+@gpu
+def test_more_rows_than_a_launch_takes():
+    """2^23 rows a launch: the rows on both sides of each border, and the last."""
+    M = (1 << 24) + 3
+    x = torch.zeros(M, 16, dtype=torch.bfloat16, device="cuda")
+    at = torch.tensor([0, (1 << 23) - 1, 1 << 23, (1 << 24) - 1, 1 << 24, M - 1], device="cuda")
+    x[at] = torch.randn(6, 16, device="cuda").to(torch.bfloat16)
+    xq, xs = ops_i8.quantize_rows(x)
+    few, fews = ops_i8.quantize_rows(x[at].contiguous())
+    assert torch.equal(xq[at], few) and torch.equal(xs[at], fews)
+    assert int(xs.count_nonzero()) == 6 and int((xq != 0).any(1).sum()) == 6
