@@ -140,30 +140,34 @@ template <int TY, int MAPS, int DQ, int DV, bool BIAS> struct FwdWave {
   }
 };
 
-// The work-group's place: b, key / value head, query head and query block.  Blocks that share K and V run on one XCD where
-// the head count allows it (blocks b and b + 8 share one); under a causal mask the longest rows come first.
+// The work-group's place: b, key / value head, query head and query block.  Heads that share K and V run on one XCD where the head
+// count allows it (work-groups b and b + 8 share one).  Without a causal mask an XCD takes one head after the other; under one the
+// longest rows of all heads come first (2 x 8 heads, 2048 tokens, two maps: 65 us, head by head 74; 16 heads, 8192 tokens: 364, 374).
 struct FwdPlace { int b, h, blk; bool ok; };
 __device__ __forceinline__ FwdPlace fwd_place(const AttnArgs& a, int nblk) {
   FwdPlace w;
-  const int G = a.H / a.Hkv, kvh = a.B * a.Hkv;
-  int bh, blk;
-  if (kvh % 8 == 0) {
+  const int G = a.H / a.Hkv, kvh = a.B * a.Hkv, heads = a.B * a.H;
+  int bh = blockIdx.x % heads, blk = blockIdx.x / heads;
+  w.ok = true;
+  if (a.causal) {
+    blk = nblk - 1 - blk;
+    if (kvh % 8 == 0) {
+      const int i = bh >> 3, kv = i / G * 8 + (bh & 7);
+      bh = kv * G + i % G;
+    }
+  } else if (kvh % 8 == 0) {
     int o, i;
     xcd_remap(blockIdx.x, nblk * G, o, i);
-    bh = (o / a.Hkv) * a.H + (o % a.Hkv) * G + i % G;
+    bh = o * G + i % G;
     blk = i / G;
     w.ok = o < kvh;
-  } else if (a.B * a.H % 8 == 0) {
+  } else if (heads % 8 == 0) {
     xcd_remap(blockIdx.x, nblk, bh, blk);
-    w.ok = bh < a.B * a.H;
-  } else {
-    bh = blockIdx.x % (a.B * a.H);
-    blk = blockIdx.x / (a.B * a.H);
-    w.ok = true;
+    w.ok = bh < heads;
   }
   w.b = bh / a.H;
   w.h = bh % a.H;
-  w.blk = a.causal ? nblk - 1 - blk : blk;
+  w.blk = blk;
   return w;
 }
 
