@@ -51,10 +51,13 @@ template <int TY, int MAPS, int DQ, int DV, int RW> struct DqLds {
   static constexpr int ALL = OUT > STAGE ? OUT : STAGE;
   static_assert(JOIN <= STAGE, "the halves' sums lie over the tiles");
 };
-// float heads of 32 keep three work-groups on a CU at the price of a few registers stored outside the loop: 52 us where two take 67
-// (136 windows of 144 tokens).
+// Work-groups on a CU that the registers are held to.  float heads of 32: three, at the price of a few registers stored outside the
+// loop (32 x 8 heads, 343 tokens: 52 us where two take 67); 16-bit heads up to 64: three (4 x 16 heads, 2048 tokens: 165 us, two 188).
+constexpr int dq_groups(int ty, int maps, int dq, int dv) {
+  return ty == TY_F32 ? (dq * maps + dv > 128 ? 1 : maps > 1 || dq > 32 ? 2 : 3) : maps > 1 || dq > 64 ? 2 : dq > 32 ? 3 : 4;
+}
 template <int TY, int MAPS, int DQ, int DV, bool BIAS, int RW>
-__global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : DQ + DV > 64 || MAPS > 1 ? 2 : 3) void attn_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, dq_groups(TY, MAPS, DQ, DV)) void attn_dq_kernel(AttnArgs a) {
   typedef typename El<TY>::T T;
   typedef typename El<TY>::Frag Frag;
   constexpr int KT = DqLds<TY, MAPS, DQ, DV, RW>::KT;
@@ -64,7 +67,7 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : D
   extern __shared__ __align__(16) char smem[];       // 2 x (K maps, V) | bias table | 4 waves: sums by distance | 4 waves: DIAG
   const BwdWork wk(a, MAPS);
   float* tab = reinterpret_cast<float*>(smem + DqLds<TY, MAPS, DQ, DV, RW>::ALL);
-  __shared__ float red[4];
+  __shared__ float red[4], mend[MAPS][4][32];
   const int nblk = wk.nblk, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, half = lane >> 5;
   const int bh = blockIdx.x % (a.B * a.H), b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
   const int blk = a.causal ? nblk - 1 - blockIdx.x / (a.B * a.H) : blockIdx.x / (a.B * a.H);
@@ -188,8 +191,84 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : D
 #pragma unroll
     for (int d = 0; d < DQ / 32; ++d) dq[p][d] = zero16();
 
+  // 32 keys from j0 on, rows 32 u of the tile: what masks and distances make of them
+  struct Keys { bool masked, left, right, plain; };
+  auto keys_at = [&](int j0) {
+    Keys w;
+    w.masked = low < j0 + 31;
+    w.left = BIAS && j0 + 31 - pmin <= -a.reach;
+    w.right = BIAS && j0 - pmax >= a.reach;
+    w.plain = !w.masked && (!BIAS || (fold && (w.left || w.right)));
+    return w;
+  };
+  auto products = [&](const char* vt, int u) {                       // X
+    Products<TY, true> xsum(zero16());
+#pragma unroll
+    for (int k = 0; k < DV / 16; ++k)
+      if (DV > 32 || k == 0 || both) xsum.add(TV::read_rows(vt, 32 * u + li, k, half), g[k]);
+    return xsum.get();
+  };
+  auto weights = [&](const char* kt, int u, int j0, const Keys& w, int p) {      // P
+    f32x16 s = zero16();
+#pragma unroll
+    for (int k = 0; k < DQ / 16; ++k)
+      if (DQ > 32 || k == 0 || both) s = El<TY>::mma(TK::read_rows(kt + p * MB, 32 * u + li, k, half), q[p][k], s);
+    if (w.plain) {
+      const float add = ((BIAS ? (w.left ? far_l : far_r) : 0.0f) - m[p]) - lg[p];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = exp2_(fmaf(s[r], c2, add));
+    } else {
+      const int last = w.masked ? limit - j0 - 4 * half : 32;
+      const float far = w.left ? far_l : far_r;
+      const bool near = BIAS && !w.left && !w.right;
+      const float* tp = tb + (j0 + 4 * half - pos);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int c = 8 * (r >> 2) + (r & 3);
+        const float e = (fmaf(s[r], c2, !BIAS ? 0.0f : near ? tp[c] : far) - m[p]) - lg[p];
+        s[r] = c <= last ? exp2_(e) : 0.0f;
+      }
+    }
+    return s;
+  };
   dma_wait<0>();
   __syncthreads();
+  if (TY != TY_F32 && nt * KT <= 128) {
+    // Rows that see few keys (the first ones under a causal mask) have large weights, by which delta's error reaches dQ and the table's
+    // near buckets: they walk their keys twice, first for that error alone.  (125 causal tokens, bfloat16: dQ 2.8e-3 off without this,
+    // 2.4e-3 with; a row of n equal weights carries 1 / sqrt(n) of it, so beyond 128 keys it is lost in the roundings of dS and dQ.)
+    for (int t = 0; t < nt; ++t) {
+      const char* kt = smem + (t & 1) * (KB + VB);
+      if (t + 1 < nt) fetch((t + 1) * KT, 1);
+      for (int u = 0; u < KT / 32; ++u) {
+        const int j0 = t * KT + 32 * u;
+        if (j0 > wave_last || (RW == 2 && u != half_of)) continue;
+        const Keys w = keys_at(j0);
+        const f32x16 x = products(kt + KB, u);
+#pragma unroll
+        for (int p = 0; p < MAPS; ++p) {
+          const f32x16 s = weights(kt, u, j0, w, p);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) err[p] = fmaf(s[r], x[r] - dl[p], err[p]);
+        }
+      }
+      dma_wait<0>();
+      __syncthreads();
+    }
+    if (nt > 1) fetch(0, 0);                                         // one tile: it still lies there
+#pragma unroll
+    for (int p = 0; p < MAPS; ++p) {
+      err[p] = half_sum(err[p]);
+      if (half == 0) mend[p][wave][li] = err[p];
+    }
+    dma_wait<0>();
+    __syncthreads();
+#pragma unroll
+    for (int p = 0; p < MAPS; ++p) {
+      dl[p] += RW == 2 ? mend[p][wave & 1][li] + mend[p][2 + (wave & 1)][li] : err[p];
+      err[p] = 0.0f;
+    }
+  }
   for (int t = 0; t < nt; ++t) {
     const char* kt = smem + (t & 1) * (KB + VB);
     const char* vt = kt + KB;
@@ -198,41 +277,16 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : D
     for (int u = 0; u < KT / 32; ++u) {
       const int j0 = t * KT + 32 * u;
       if (j0 > wave_last || (RW == 2 && u != half_of)) continue;
-      const bool masked = low < j0 + 31;
-      const bool left = BIAS && j0 + 31 - pmin <= -a.reach, right = BIAS && j0 - pmax >= a.reach;
-      const bool plain = !masked && (!BIAS || (fold && (left || right)));
-      Products<TY, true> xsum(zero16());
-#pragma unroll
-      for (int k = 0; k < DV / 16; ++k)
-        if (DV > 32 || k == 0 || both) xsum.add(TV::read_rows(vt, 32 * u + li, k, half), g[k]);
-      const f32x16 x = xsum.get();
+      const Keys w = keys_at(j0);
+      const f32x16 x = products(vt, u);
       Frag df[MAPS][2];
 #pragma unroll
       for (int p = 0; p < MAPS; ++p) {
-        f32x16 s = zero16();
-#pragma unroll
-        for (int k = 0; k < DQ / 16; ++k)
-          if (DQ > 32 || k == 0 || both) s = El<TY>::mma(TK::read_rows(kt + p * MB, 32 * u + li, k, half), q[p][k], s);
-        if (plain) {
-          const float add = ((BIAS ? (left ? far_l : far_r) : 0.0f) - m[p]) - lg[p];
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = exp2_(fmaf(s[r], c2, add));
-        } else {
-          const int last = masked ? limit - j0 - 4 * half : 32;
-          const float far = left ? far_l : far_r;
-          const bool near = BIAS && !left && !right;
-          const float* tp = tb + (j0 + 4 * half - pos);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int c = 8 * (r >> 2) + (r & 3);
-            const float e = (fmaf(s[r], c2, !BIAS ? 0.0f : near ? tp[c] : far) - m[p]) - lg[p];
-            s[r] = c <= last ? exp2_(e) : 0.0f;
-          }
-        }
+        f32x16 s = weights(kt, u, j0, w, p);
         if constexpr (BIAS) {
-          if (left || right) {
-            const float w = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7])) + (((s[8] + s[9]) + (s[10] + s[11])) + ((s[12] + s[13]) + (s[14] + s[15])));
-            if (left) p_l += w; else p_r += w;
+          if (w.left || w.right) {
+            const float sum = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7])) + (((s[8] + s[9]) + (s[10] + s[11])) + ((s[12] + s[13]) + (s[14] + s[15])));
+            if (w.left) p_l += sum; else p_r += sum;
           }
         }
         const float sg = (MAPS == 2 && p == 1) ? -lam : 1.0f;
@@ -246,8 +300,8 @@ __global__ __launch_bounds__(256, (TY == TY_F32 && DQ * MAPS + DV > 128) ? 1 : D
         const float all = (tot[0] + tot[1]) * irs;
         err[p] += all;
         if constexpr (BIAS) {
-          if (left) sum_l += all;
-          else if (right) sum_r += all;
+          if (w.left) sum_l += all;
+          else if (w.right) sum_r += all;
           else {
             // Sums by distance, 16 keys at a time: the tile as rows of 32 with 15 zeros between them (row k at 47 k, the zeros stay),
             // where the entries of one distance, k - q, lie 48 apart; lane u < 47 adds up those of distance 15 - u.  (LDS atomics

@@ -225,9 +225,9 @@ __device__ __forceinline__ f32x16 zero16() {
 
 // The sum of a few products from ``start`` on.  float: the matrix pipe cuts off what lies below its largest term towards minus
 // infinity.  A start far larger than the products (an exponent's maximum) would cost them bits, so the vector pipe adds it at the end
-// (777 tokens: dK and dV 1.3e-6 off from such a start, 6e-7 so).  With APART the products of the upper parts, which lose nothing to
-// speak of, have an accumulator of their own beside the small ones: the mean error of an instruction, -3e-8, otherwise adds up over the
-// thousands of pairs of a bias table's bucket (its gradient 1.8e-6 off, and 3.5e-7 so).
+// (777 tokens: dK and dV 1.3e-6 off from such a start, 6e-7 so).  APART, from zero: the products of the upper parts, which lose nothing
+// to speak of, have an accumulator of their own beside the small ones; the mean error of an instruction, -3e-8, otherwise adds up over
+// the thousands of pairs of a bias table's bucket (its gradient 1.8e-6 off, and 3.5e-7 so).
 template <int TY, bool APART = false> struct Products {
   f32x16 sum;
   __device__ __forceinline__ Products(f32x16 start) : sum(start) {}
@@ -235,8 +235,8 @@ template <int TY, bool APART = false> struct Products {
   __device__ __forceinline__ f32x16 get() const { return sum; }
 };
 template <bool APART> struct Products<TY_F32, APART> {
-  f32x16 start, sum, rest;
-  __device__ __forceinline__ Products(f32x16 start) : start(start), sum(zero16()), rest(zero16()) {}
+  f32x16 rest, sum;            // rest: the start; APART: the small products
+  __device__ __forceinline__ Products(f32x16 start) : rest(start), sum(zero16()) {}
   __device__ __forceinline__ void add(Split8 a, Split8 b) {
     if (APART) {
       rest = El<TY_F32>::mma_small(a, b, rest);
@@ -245,7 +245,7 @@ template <bool APART> struct Products<TY_F32, APART> {
       sum = El<TY_F32>::mma(a, b, sum);
     }
   }
-  __device__ __forceinline__ f32x16 get() const { return (APART ? sum + rest : sum) + start; }
+  __device__ __forceinline__ f32x16 get() const { return sum + rest; }
 };
 
 // A wave's 32 x COLS result, row li on lane li, to 32 rows of a strided matrix (those below ``rows``, elements below ``cols``): through
