@@ -7,7 +7,9 @@
 //
 // No atomics and no Lq x Lk array: every sum has one owner and a fixed order.
 //   attn_dq_kernel   a wave owns 32 queries and walks the keys: delta, dQ, the table's gradient by distance
+//                    (4 x 16 heads of 64, 2048 tokens, bfloat16: 165 us, vector pipe 54 % of the cycles, matrix 29, LDS 30)
 //   attn_dkv_kernel  a wave owns 32 keys and walks the queries of all heads that share them: dK, dV
+//                    (the same: 186 us, matrix 35, vector 36, LDS 37; heads beyond 64: one work-group on a CU, by registers)
 //   *_dw_kernel      sums the work-groups' parts of the learned weights' gradient
 // The price is that scores and X are computed twice (7 products instead of 5); what it buys is that gradients are the same from
 // run to run and that dQ (f32, Lq x D a head and key block) is never read back.
