@@ -235,7 +235,8 @@ __global__ __launch_bounds__(256, dq_groups(TY, MAPS, DQ, DV)) void attn_dq_kern
   };
   dma_wait<0>();
   __syncthreads();
-  if (TY != TY_F32 && nt * KT <= 128) {
+  if (TY != TY_F32 && nt <= 2) {
+    static_assert(TY == TY_F32 || KT == 64, "two tiles of 64 keys: the first still lies in its stage afterwards");
     // Rows that see few keys (the first ones under a causal mask) have large weights, by which delta's error reaches dQ and the table's
     // near buckets: they walk their keys twice, first for that error alone.  (125 causal tokens, bfloat16: dQ 2.8e-3 off without this,
     // 2.4e-3 with; a row of n equal weights carries 1 / sqrt(n) of it, so beyond 128 keys it is lost in the roundings of dS and dQ.)
@@ -257,13 +258,11 @@ __global__ __launch_bounds__(256, dq_groups(TY, MAPS, DQ, DV)) void attn_dq_kern
       dma_wait<0>();
       __syncthreads();
     }
-    if (nt > 1) fetch(0, 0);                                         // one tile: it still lies there
 #pragma unroll
     for (int p = 0; p < MAPS; ++p) {
       err[p] = half_sum(err[p]);
       if (half == 0) mend[p][wave][li] = err[p];
     }
-    dma_wait<0>();
     __syncthreads();
 #pragma unroll
     for (int p = 0; p < MAPS; ++p) {
