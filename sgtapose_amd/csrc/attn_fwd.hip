@@ -364,9 +364,10 @@ __global__ __launch_bounds__(256) void attn_step_kernel(AttnArgs a, int splits) 
   wv.c2 = a.scale * LOG2E;
   wv.both = a.D > 16;
   if constexpr (BIAS) {
-    // the tables are read by tiles within ``reach`` of the queries only: most parts of a long cache have none
+    // the tables are read by tiles within ``reach`` of the queries only (whole tiles: the last one begins at k1 - 1 at the latest and has
+    // KT keys, seen or not): most parts of a long cache have none
     const int n = bias_size(a.reach);
-    if (k1 - 1 - wv.pmin > -a.reach && k0 - wv.pmax < a.reach)
+    if (k1 - 1 + KT - 1 - wv.pmin > -a.reach && k0 - wv.pmax < a.reach)
       for (int x = 0; x < G; ++x) fill_bias<TY>(a, tabs + x * n, hk * G + x, tid, 256);
     wv.tab = tabs + (row < R ? g : 0) * n + a.reach + BIAS_PAD;
     wv.far_l = bias_log2<TY>(a, -a.reach, h);

@@ -642,3 +642,17 @@ def test_positions_too_far_apart_are_refused():
     for args in ((far, near, near), (near, far, near), (near, near, far)):
         with pytest.raises(SgtaHipError, match="bytes apart"):
             ops_attn.rel_attention(*args, table)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ALL, ids=NAMES.get)
+def test_keys_beyond_the_reach_in_a_tile_that_is_not(dtype):
+    """Few keys, all farther from the query than any bucket of its own, in a tile whose empty rest is nearer.  Calls with another table,
+    whose values are large, come between, so that nothing left in LDS by an equal one helps."""
+    other = Case(1, dtype, 8, 1, 40, 64, 8, 32, buckets=4, far=3, q_start=[20] * 8)
+    other.w[:] = 100.0 * (1 + torch.arange(4)[:, None])
+    for n, (Lq, kv_len, q_start) in enumerate([(1, 13, 30), (1, 1, 17), (2, 1, 9), (5, 1, 5), (1, 33, 50), (23, 1, 20), (2, 31, 36), (1, 130, 150)]):
+        for causal in (False, True):
+            forward(other)
+            check_both(Case(1, dtype, 3, Lq, max(71, kv_len), 3, 3, 32, causal=causal, buckets=4, far=3, kv_len=[kv_len] * 3,
+                            q_start=[q_start] * 3, seed=n))
