@@ -109,6 +109,9 @@ __global__ __launch_bounds__(256, dq_groups(TY, MAPS, DQ, DV)) void attn_dq_kern
   // the row's operands, delta and largest |dO|
   Frag q[MAPS][DQ / 16], g[DV / 16];
   float m[MAPS], lg[MAPS], dl[MAPS], top = 0.0f;
+  // float: every other row's X is computed with its sign turned, so that what is left of the cut-off's mean error cancels in sums over
+  // rows (lambda's gradient, the table's)
+  const float sx = TY == TY_F32 && (li & 1) ? -1.0f : 1.0f;
   {
     const T* qp = (const T*)a.q + b * a.sq[0] + row * a.sq[1] + h * a.sq[2];
 #pragma unroll
@@ -127,7 +130,8 @@ __global__ __launch_bounds__(256, dq_groups(TY, MAPS, DQ, DV)) void attn_dq_kern
       const int d = 16 * s + 8 * half;
       const bool in = ok && d < a.Dv;
       const typename El<TY>::Raw gr = global_raw<TY>(gp + d, in), o = global_raw<TY>(op + d, in);
-      g[s] = El<TY>::frag_of(gr);
+      if constexpr (TY == TY_F32) g[s] = El<TY>::frag_of(gr * sx);
+      else g[s] = El<TY>::frag_of(gr);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         s1 = fmaf((float)gr[e], (float)o[e], s1);
@@ -294,7 +298,7 @@ __global__ __launch_bounds__(256, dq_groups(TY, MAPS, DQ, DV)) void attn_dq_kern
         float tot[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const float d = s[r] * (TY == TY_F16 ? fmaf(x[r], rs, -dl[p] * rs) : x[r] - dl[p]);
+          const float d = s[r] * (TY == TY_F16 ? fmaf(x[r], rs, -dl[p] * rs) : TY == TY_F32 ? fmaf(x[r], sx, -dl[p]) : x[r] - dl[p]);
           s[r] = (MAPS == 2 && p == 1) ? d * sg : d;
           tot[r & 1] += d;
         }
