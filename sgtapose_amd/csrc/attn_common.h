@@ -169,11 +169,17 @@ template <int TY, int COLS> struct Tile {
 
 // Global memory -> LDS, 16 bytes a lane, to LDS byte ``at`` + 16 lane.  In assembly although there is a builtin: of that the
 // compiler assumes that any transposing LDS read may see its data, and waits for all of it (the NEXT tile) before each of them.
-// It has no result register; what was loaded is read only after dma_wait and a barrier.
+// It has no result register; what was loaded is read only after dma_wait and a barrier.  Between the write of M0 and a load into LDS the
+// hardware asks for one wait state, which the compiler does not add inside assembly (tests/test_wait_states.py looks for it, and for the
+// five between a vector instruction's write of a scalar register and the load, in the built library).  M0 stays on the clobber list,
+// so that the compiler takes no value of its own for still there; its remark, that it does not save the register, is what is wanted.
 #if defined(__HIP_DEVICE_COMPILE__)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, unsigned off, unsigned at) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(rs) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(rs) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 #endif
 
 // Rows of a strided matrix into a Tile by NT threads, straight into LDS (no registers, no LDS store instructions): a wave writes
