@@ -195,6 +195,7 @@ __global__ __launch_bounds__(256, dq_groups(TY, MAPS, DQ, DV)) void attn_dq_kern
     diag = tab + 5 * wk.nrel + wave * DIAG + 15;
   }
   const float c2 = a.scale * LOG2E;
+  const float c2r = fabsf(m[0]) < BIAS_FOLD ? c2 : 0.0f;             // a bias beyond absorbs its row's scores
   const bool both = a.D > 16;                         // DQ = 32: the second 16 of the head's elements are not all padding
   const int wave_last = row0 >= nq ? -1 : a.causal ? min(seen - 1, st + min(row0 + 31, nq - 1)) : seen - 1;
 
@@ -233,13 +234,13 @@ __global__ __launch_bounds__(256, dq_groups(TY, MAPS, DQ, DV)) void attn_dq_kern
       for (int r = 0; r < 16; ++r) s[r] = EXACT ? exp2_(fmaf(s[r], c2, add)) * lg[p] : exp2_(fmaf(s[r], c2, add));
     } else {
       const int last = w.masked ? limit - j0 - 4 * half : 32;
-      const float far = w.left ? far_l : far_r;
       const bool near = BIAS && !w.left && !w.right;
+      const float far = (w.left ? far_l : far_r) - m[p];
       const float* tp = tb + (j0 + 4 * half - pos);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int c = 8 * (r >> 2) + (r & 3);
-        const float e = fmaf(s[r], c2, !BIAS ? 0.0f : near ? tp[c] : far) - m[p];
+        const float e = BIAS ? fmaf(s[r], c2r, near ? tp[c] - m[p] : far) : s[r] * c2 - m[p];
         s[r] = c > last ? 0.0f : EXACT ? exp2_(e) * lg[p] : exp2_(e - lg[p]);
       }
     }
@@ -534,7 +535,7 @@ __global__ __launch_bounds__(256, (MAPS * DQ + DV > 128 || (TY == TY_F32 && MAPS
   for (int d = 0; d < DV / 32; ++d) dv[d] = zero16();
 
   float far_l = 0.0f, far_r = 0.0f;
-  bool fold = true;
+  bool fold = true;                                  // both small enough to be added to a start that -m is already in
   int h = hk * G, r0 = q_first;
   if (steps > 0) put(0);
   for (int it = 0; it < steps; ++it) {
@@ -543,7 +544,7 @@ __global__ __launch_bounds__(256, (MAPS * DQ + DV > 128 || (TY == TY_F32 && MAPS
       fill_bias<TY>(a, tab, h, tid, 256);
       far_l = bias_log2<TY>(a, -a.reach, h);
       far_r = bias_log2<TY>(a, a.reach, h);
-      fold = fabsf(far_l) < BIAS_FOLD && fabsf(far_r) < BIAS_FOLD;
+      fold = fabsf(far_l) < BIAS_LARGE && fabsf(far_r) < BIAS_LARGE;
     }
     if (it == 0) dma_wait<0>();
     if (it == 0 || (BIAS && r0 == q_first)) __syncthreads();
@@ -603,8 +604,9 @@ __global__ __launch_bounds__(256, (MAPS * DQ + DV > 128 || (TY == TY_F32 && MAPS
             const f32x4 mm = *reinterpret_cast<const f32x4*>(sp + 2 * QT), ll = *reinterpret_cast<const f32x4*>(sp + 3 * QT);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const float e = (fmaf(s[4 * c + r], c2, !BIAS ? 0.0f : near ? tp[-(8 * c + r)] : far) - mm[r]) - ll[r];
-              s[4 * c + r] = 8 * c + r >= first ? exp2_(e) : 0.0f;
+              // a bias beyond BIAS_FOLD absorbs its row's scores
+              const float e = BIAS ? fmaf(s[4 * c + r], fabsf(mm[r]) < BIAS_FOLD ? c2 : 0.0f, (near ? tp[-(8 * c + r)] : far) - mm[r]) : s[4 * c + r] * c2 - mm[r];
+              s[4 * c + r] = 8 * c + r >= first ? exp2_(e - ll[r]) : 0.0f;
             }
           }
         }

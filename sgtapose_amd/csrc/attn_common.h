@@ -324,12 +324,34 @@ template <int TY> __device__ __forceinline__ float bias_log2(const AttnArgs& a, 
   const float s = t * LOG2E;
   return (fabsf(s) == INFINITY && fabsf(t) != INFINITY) ? copysignf(3.402823466e38f, s) : s;
 }
-template <int TY> __device__ __forceinline__ void fill_bias(const AttnArgs& a, float* tab, int h, int tid, int nt) {
-  const int n = bias_size(a.reach);
-  for (int i = tid; i < n; i += nt) tab[i] = bias_log2<TY>(a, i - a.reach - BIAS_PAD, h);
+// A softmax does not see a constant, so what a large bias has in common with a row's maximum is taken off before the score is added, in
+// both directions: fma(s, c2, bias - maximum).  (Added first, a value of -1e4 costs a weight 5e-4 of itself, one of -1e6 8 %, and the
+// weights of the backward pass no longer sum to one.)  Two limits, in units of log2:
+//   BIAS_FOLD   from here on a bias is added first and absorbs the scores: keys that only such a value is left for weigh evenly (a type's
+//               lowest value).  Below it a maximum, held in f32, is off by at most 64, and the weights with it by 2^64, which f32 and
+//               bfloat16 hold; IEEE half tables end at 2^17.
+//   BIAS_LARGE  heads with such a value take their near tiles' largest visible bias off first in the forward pass (one more read and two
+//               instructions an element); below it the sum's rounding, 2^-20 of a weight, is that of any score of the size.  So do the
+//               far tiles of attn_dkv_kernel, whose scores otherwise start from -maximum and have the far value added at the end.
+#define BIAS_FOLD 2147483648.0f
+#define BIAS_LARGE 16.0f
+// A copy that the compiler takes for another number: branches that each compare it with an unrolled tile's columns otherwise get one set
+// of 16 to 32 lane masks ahead of them all, more than the scalar registers hold (5 to 9 % of the training cases).
+__device__ __forceinline__ int another(int x) {
+  asm("" : "+v"(x));
+  return x;
 }
-// beyond this a bias absorbs the scores it is added to: such tiles add it to each score instead of folding it into the exponent
-#define BIAS_FOLD 1e30f
+// -> whether this thread met a finite value of BIAS_LARGE or more
+template <int TY> __device__ __forceinline__ bool fill_bias(const AttnArgs& a, float* tab, int h, int tid, int nt) {
+  const int n = bias_size(a.reach);
+  bool large = false;
+  for (int i = tid; i < n; i += nt) {
+    const float t = bias_log2<TY>(a, i - a.reach - BIAS_PAD, h);
+    tab[i] = t;
+    large |= fabsf(t) >= BIAS_LARGE && fabsf(t) < INFINITY;
+  }
+  return large;
+}
 
 // lets a kernel use up to 158 KB of dynamic LDS on the current device (once a device; 2 KB of the 160 are left for static arrays),
 // refuses more

@@ -30,6 +30,7 @@ template <int TY, int MAPS, int DQ, int DV, bool BIAS> struct FwdWave {
   const float* tab;            // BIAS: this lane's head's table, at rel = 0
   float far_l, far_r;          // its values left and right of ``reach``
   bool fold;                   // both may be folded into the exponent
+  bool large;                  // some value of the table is BIAS_LARGE or more
   float c2;                    // scale in log2 units
   bool both;                   // DQ = 32: the second 16 of the head's elements are not all padding
 
@@ -86,8 +87,8 @@ template <int TY, int MAPS, int DQ, int DV, bool BIAS> struct FwdWave {
     const int li = lane & 31, half = lane >> 5;
     const bool masked = low < j0 + NK - 1;
     const bool left = BIAS && j0 + NK - 1 - pmin <= -reach, right = BIAS && j0 - pmax >= reach;
-    // plain: every query sees every key and the bias is one value, which goes into the exponent
-    const bool plain = !masked && (!BIAS || (fold && (left || right)));
+    // folded: the bias is one value, which goes into the exponent; plain: every query sees every key, too
+    const bool folded = BIAS && fold && (left || right), plain = !masked && (!BIAS || folded);
     Frag pf[MAPS][NK / 16];
 #pragma unroll
     for (int p = 0; p < MAPS; ++p) {
@@ -101,23 +102,54 @@ template <int TY, int MAPS, int DQ, int DV, bool BIAS> struct FwdWave {
       }
       float al;
       bool grown;
-      if (plain) {
+      const int last = masked ? limit - j0 - 4 * half : NK;
+      if (plain || folded) {
+        if (masked) {
+          const int to = another(last);
+#pragma unroll
+          for (int u = 0; u < NS; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[u][r] = 32 * u + 8 * (r >> 2) + (r & 3) <= to ? s[u][r] : -INFINITY;
+        }
         al = weights<NS>(s, p, c2, !BIAS ? 0.0f : left ? far_l : far_r, grown);
       } else {
-        const int last = masked ? limit - j0 - 4 * half : NK;
-        const float far = left ? far_l : far_r;
-        const float* t = tab + (j0 + 4 * half - pos);
         const bool near = BIAS && !left && !right;
+        const float* t = tab + (j0 + 4 * half - pos);
+        const float far = left ? far_l : far_r, cf = !BIAS || fabsf(far) < BIAS_FOLD ? c2 : 0.0f;
+        float add = 0.0f;
+        if (near && large) {
+          int to = another(last);
+          add = -INFINITY;                             // the largest bias that this row sees in the tile
 #pragma unroll
-        for (int u = 0; u < NS; ++u)
+          for (int u = 0; u < NS; ++u)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int c = 32 * u + 8 * (r >> 2) + (r & 3);
-            float x = s[u][r] * c2;
-            if (BIAS) x = fmaf(s[u][r], c2, near ? t[c] : far);
-            s[u][r] = c <= last ? x : -INFINITY;
-          }
-        al = weights<NS>(s, p, 1.0f, 0.0f, grown);
+            for (int r = 0; r < 16; ++r) {
+              const int c = 32 * u + 8 * (r >> 2) + (r & 3);
+              add = fmaxf(add, c <= to ? t[c] : -INFINITY);
+            }
+          add = half_max(add);
+          add = fabsf(add) < BIAS_FOLD ? add : 0.0f;
+          to = another(to);
+#pragma unroll
+          for (int u = 0; u < NS; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int c = 32 * u + 8 * (r >> 2) + (r & 3);
+              const float x = fmaf(s[u][r], fabsf(t[c]) < BIAS_FOLD ? c2 : 0.0f, t[c] - add);
+              s[u][r] = c <= to ? x : -INFINITY;
+            }
+        } else {
+#pragma unroll
+          for (int u = 0; u < NS; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int c = 32 * u + 8 * (r >> 2) + (r & 3);
+              float x = s[u][r] * c2;
+              if (BIAS) x = fmaf(s[u][r], near ? c2 : cf, near ? t[c] : far);
+              s[u][r] = c <= last ? x : -INFINITY;
+            }
+        }
+        al = weights<NS>(s, p, 1.0f, add, grown);
       }
       if (__any(grown)) {
 #pragma unroll
@@ -185,6 +217,7 @@ __global__ __launch_bounds__(256, TY == TY_F32 && MAPS * DQ + DV > 128 ? 1 : 2) 
   constexpr int MB = KT * DQ * (int)sizeof(T), KB = MAPS * MB, VB = KT * DV * (int)sizeof(T);
   extern __shared__ __align__(16) char smem[];       // 2 x (K maps, V), then the bias table
   float* tab = reinterpret_cast<float*>(smem + 2 * (KB + VB));       // nothing reads it when the epilogue lies over it
+  __shared__ int large[4];
   const FwdPlace w = fwd_place(a, nblk);
   if (!w.ok) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, half = lane >> 5;
@@ -222,7 +255,8 @@ __global__ __launch_bounds__(256, TY == TY_F32 && MAPS * DQ + DV > 128 ? 1 : 2) 
   wv.c2 = a.scale * LOG2E;
   wv.both = a.D > 16;
   if constexpr (BIAS) {
-    fill_bias<TY>(a, tab, h, tid, 256);
+    const bool l = __any(fill_bias<TY>(a, tab, h, tid, 256));
+    if (lane == 0) large[wave] = l;
     wv.tab = tab + a.reach + BIAS_PAD;
     wv.far_l = bias_log2<TY>(a, -a.reach, h);
     wv.far_r = bias_log2<TY>(a, a.reach, h);
@@ -232,6 +266,7 @@ __global__ __launch_bounds__(256, TY == TY_F32 && MAPS * DQ + DV > 128 ? 1 : 2) 
 
   dma_wait<0>();
   __syncthreads();
+  if constexpr (BIAS) wv.large = large[0] | large[1] | large[2] | large[3];
   for (int t = 0; t < nt; ++t) {
     const char* kt = smem + (t & 1) * (KB + VB);
     if (t + 1 < nt) fetch((t + 1) * KT, (t & 1) ^ 1);
@@ -333,6 +368,7 @@ __global__ __launch_bounds__(256) void attn_step_kernel(AttnArgs a, int splits) 
   const bool ok = row < R && i < nq;
   char* mine = smem + wave * L::BUFS * (L::KB + L::VB);
   float* tabs = reinterpret_cast<float*>(smem + L::LDS);
+  __shared__ int large[4];
 
   // each part ends where the next begins
   const int seen = a.causal ? min(nk, max(st + nq, 0)) : nk;
@@ -367,13 +403,17 @@ __global__ __launch_bounds__(256) void attn_step_kernel(AttnArgs a, int splits) 
     // the tables are read by tiles within ``reach`` of the queries only (whole tiles: the last one begins at k1 - 1 at the latest and has
     // KT keys, seen or not): most parts of a long cache have none
     const int n = bias_size(a.reach);
+    bool l = false;
     if (k1 - 1 + KT - 1 - wv.pmin > -a.reach && k0 - wv.pmax < a.reach)
-      for (int x = 0; x < G; ++x) fill_bias<TY>(a, tabs + x * n, hk * G + x, tid, 256);
+      for (int x = 0; x < G; ++x) l |= fill_bias<TY>(a, tabs + x * n, hk * G + x, tid, 256);
+    l = __any(l);
+    if (lane == 0) large[wave] = l;
     wv.tab = tabs + (row < R ? g : 0) * n + a.reach + BIAS_PAD;
     wv.far_l = bias_log2<TY>(a, -a.reach, h);
     wv.far_r = bias_log2<TY>(a, a.reach, h);
     wv.fold = !__any(fabsf(wv.far_l) >= BIAS_FOLD || fabsf(wv.far_r) >= BIAS_FOLD);
     __syncthreads();
+    wv.large = large[0] | large[1] | large[2] | large[3];
   }
   for (int buf = 0; j0 < k1; j0 += 4 * KT) {
     const char* now = mine + buf * (L::KB + L::VB);
