@@ -771,6 +771,7 @@ template <int TY, int MAPS, int DQ, int DV, bool BIAS> static int launch_bwd(con
 static int bwd_check(const AttnArgs* a, int maps) {
   if (int e = attn_check(a, maps)) return e;
   if (!a->dout || !a->dq || !a->dk || !a->dv || !a->dw || !a->stats || !a->ws || (maps == 2 && !a->out2)) return SGTA_EBADARG;
+  if (maps == 1 && (long)a->H * a->num_buckets >= MAX_GROUPS) return SGTA_ETOOBIG;
   if (a->ws_floats < BwdWork(*a, maps).total || (uintptr_t)a->ws % 16) return SGTA_EBADARG;
   const int al = a->dtype == TY_F32 ? 4 : 8;
   const long* s[] = {a->sdo, a->sdq, a->sdk, a->sdv};

@@ -35,6 +35,7 @@ from . import _lib
 raw_stream = torch._C._cuda_getCurrentRawStream      # (device index) -> the current stream's handle; 2 us less a call than the Stream object
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 MAX_PITCH = 1 << 24            # bytes from one position to the next
+MAX_GROUPS = 1 << 24           # blocks of 128 positions of all sequences and heads
 MAX_REACH = 1024               # distances that may have buckets of their own (the kernels keep them in LDS)
 
 
@@ -131,6 +132,8 @@ def _plan(maps, qs, qst, ks, kst, vs, vst, dtype, causal, scale, w_shape, max_di
         _fail("head sizes %d, %d: multiples of 8 up to %d, %d%s", D, Dv, *most, ", equal" if maps == 1 else "")
     if max(Lq, Lk) >= 1 << 29:
         _fail("sequences of %d, %d: below 2^29", Lq, Lk)
+    if B * H * ((max(Lq, Lk) + 127) // 128) >= MAX_GROUPS:
+        _fail("%d sequences of %d, %d with %d heads: B * H * ceil(longest / 128) stays below 2^24", B, Lq, Lk, H)
     if scale is None:
         scale = D ** -0.5
     if not (scale > 0 and math.isfinite(scale)):

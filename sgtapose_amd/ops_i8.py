@@ -14,6 +14,7 @@ import torch
 from . import _lib
 from .ops_attn import DTYPES, _fail, raw_stream
 
+MAX_COUNT = (1 << 31) - 1
 MAX_K = 131071                 # 127 * 128 * K stays below 2^31
 
 
@@ -25,6 +26,8 @@ def _rows(name, shape, stride, dtype, dtypes, want=None):
     M, K = shape
     if M < 1 or K < 1:
         _fail("%s is empty: %s", name, tuple(shape))
+    if max(M, K) > MAX_COUNT:
+        _fail("%s: %s, at most %d rows and columns (the kernels count in 32 bits)", name, tuple(shape), MAX_COUNT)
     if (K > 1 and stride[1] != 1) or (M > 1 and stride[0] < K):
         _fail("%s: rows of consecutive elements that do not overlap expected, strides %s", name, tuple(stride))
     return stride[0] if M > 1 else max(K, stride[0])
