@@ -278,15 +278,25 @@ def diff_attention(q, k, v, lam, out=None, *, lam_init=0.8, causal=False, scale=
     return _forward("sgta_diff_attn_fwd", 2, a, q, out, q_len, save)
 
 
+def _saved(stats, out2, maps, shape, like):
+    """Checks what the forward call kept: the kernels read it as it was written, whole and contiguous."""
+    B, Lq, H, _ = shape
+    ok = [stats is not None and tuple(stats.shape) == (maps, B, H, Lq, 2) and stats.dtype == torch.float32 and stats.device == like.device
+          and stats.is_contiguous(), (out2 is None) == (maps == 1)]
+    if all(ok) and maps == 2:
+        ok.append(tuple(out2.shape) == tuple(shape) and out2.dtype == like.dtype and out2.device == like.device and out2.is_contiguous()
+                  and out2.data_ptr() % 16 == 0)
+    if not all(ok):
+        _fail("saved does not come from a forward call of this shape")
+
+
 def _backward(name, maps, a, like, dout, w, out, saved, grads, q_len, kv_len):
     mp = (2,) if maps == 2 else ()
     stats, out2 = saved
     shape = (a.B, a.Lq, a.H, a.Dv)
     _set_strides(a, "sdo", _like("dout", dout, shape, like), False)
     _set_strides(a, "so", _like("out", out, shape, like), False)
-    if tuple(stats.shape) != (maps, a.B, a.H, a.Lq, 2) or stats.device != like.device or (out2 is None) != (maps == 1) or (
-            maps == 2 and (tuple(out2.shape) != shape or out2.dtype != like.dtype)):
-        _fail("saved does not come from a forward call of this shape")
+    _saved(stats, out2, maps, shape, like)
     a.dout, a.out, a.stats = dout.data_ptr(), out.data_ptr(), stats.data_ptr()
     if maps == 2:
         a.out2 = out2.data_ptr()
