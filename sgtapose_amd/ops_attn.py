@@ -19,6 +19,9 @@ log2); beyond, down to a type's lowest value, they absorb the scores, so that a 
 Within the lengths a value that is not finite may also reach positions from which the mask hides it (0 times infinity), as in the
 plain products.  float32 operands are split into three bfloat16 numbers, so that an infinity among them gives not-a-numbers.
 
+Nothing is recorded for autograd: outside ``torch.no_grad()`` operands that require a gradient are refused unless ``save=True`` says that
+the caller takes the backward operator.  Its ``dout`` is laid out as the other operands are (an expanded one: ``.contiguous()`` first).
+
 Everything is enqueued on the current stream of the tensors' device; workspaces come from torch's allocator anew in each call, so
 calls on several streams and calls captured into several graphs do not share any.  Outputs share no memory with each other or with
 what a call reads.  ``rel_attention`` puts the table of buckets on the device at its first call with given settings, which cannot be
@@ -246,6 +249,13 @@ def _meta(kernel, a, maps, products):
             "bytes": size * (a.B * a.Lq * a.H * (maps * a.D + a.Dv) + a.B * a.Lk * a.Hkv * (maps * a.D + a.Dv))}
 
 
+def _no_graph(save, *tensors):
+    """These operators record nothing for autograd: a result that looks as if it did would train without its share of the gradient."""
+    if not save and torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        _fail("an operand requires a gradient, which this call does not record: call it under torch.no_grad(), or with save=True and the "
+              "backward operator (inside an autograd.Function, say)")
+
+
 def _forward(name, maps, a, like, out, q_len, save):
     shape = (a.B, a.Lq, a.H, a.Dv)
     out = _output(a, "out", "so", out, shape, like, q_len is not None)
@@ -266,6 +276,7 @@ def rel_attention(q, k, v, table, out=None, *, max_distance=128, bidirectional=T
 
     ``table`` [num_buckets, H] is the learned bias; buckets as ``relative_buckets(num_buckets, max_distance, bidirectional)``.
     ``scale`` None: D ** -0.5.  ``save``: returns (out, saved) for ``rel_attention_bwd``."""
+    _no_graph(save, q, k, v, table)
     a = _operands(1, q, k, v, table, causal, scale, q_len, kv_len, q_start, int(max_distance), bool(bidirectional))
     return _forward("sgta_rel_attn_fwd", 1, a, q, out, q_len, save)
 
@@ -274,6 +285,7 @@ def diff_attention(q, k, v, lam, out=None, *, lam_init=0.8, causal=False, scale=
     """(softmax(scale q1 k1^T) - lambda softmax(scale q2 k2^T)) v; ``lam`` [4, D] holds the learned vectors of
     lambda = exp(lam[0].lam[1]) - exp(lam[2].lam[3]) + lam_init, one for all heads.  V is read once for both maps.
     ``save``: returns (out, saved) for ``diff_attention_bwd``."""
+    _no_graph(save, q, k, v, lam)
     a = _operands(2, q, k, v, lam, causal, scale, q_len, kv_len, q_start, lam_init=float(lam_init))
     return _forward("sgta_diff_attn_fwd", 2, a, q, out, q_len, save)
 
