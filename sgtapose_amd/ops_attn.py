@@ -238,15 +238,18 @@ def _enqueue(name, a, device, ws_name, maps, meta):
     _lib.call(name, ctypes.byref(a), raw_stream(device.index), meta=meta)
 
 
-def _meta(kernel, a, maps, products):
-    """Algorithmic work for the live profile: ``products`` of D and of Dv per pair of positions (full, unmasked lengths)."""
+def _meta(kernel, a, maps, backward=False):
+    """Work for the live profile (full, unmasked lengths): ``flops`` of the formulas' products of D and of Dv per pair of positions,
+    ``exec_flops`` with the scores and dO V^T that the backward kernels compute twice, ``bytes`` with each tensor once."""
     if _lib.PROFILE is None:
         return None
     pairs = 2.0 * a.B * a.H * a.Lq * a.Lk * (0.5 if a.causal and a.Lq == a.Lk else 1.0)
-    flops = pairs * (products[0] * a.D + products[1] * a.Dv)
+    need, does = ((3 * maps, 2), (4 * maps, 3)) if backward else ((maps, maps),) * 2
+    flops, execs = (pairs * (d * a.D + dv * a.Dv) for d, dv in (need, does))
     size = 4 if a.dtype == 0 else 2
-    return {"kernel": kernel, "flops": flops, "exec_flops": flops,
-            "bytes": size * (a.B * a.Lq * a.H * (maps * a.D + a.Dv) + a.B * a.Lk * a.Hkv * (maps * a.D + a.Dv))}
+    q, kv, o = a.B * a.Lq * a.H * maps * a.D, a.B * a.Lk * a.Hkv * (maps * a.D + a.Dv), a.B * a.Lq * a.H * a.Dv
+    count = 2 * q + 2 * kv + (maps + 1) * o if backward else q + kv + o          # and each gradient; out, the second map's, dout
+    return {"kernel": kernel, "flops": flops, "exec_flops": execs, "bytes": size * count}
 
 
 def _no_graph(save, *tensors):
@@ -266,7 +269,7 @@ def _forward(name, maps, a, like, out, q_len, save):
         if maps == 2:
             out2 = torch.empty(shape, dtype=like.dtype, device=like.device)
             a.out2 = out2.data_ptr()
-    _enqueue(name, a, like.device, "sgta_attn_fwd_ws_floats", maps, _meta(name, a, maps, (maps, maps)))
+    _enqueue(name, a, like.device, "sgta_attn_fwd_ws_floats", maps, _meta(name, a, maps))
     return (out, (stats, out2)) if save else out
 
 
@@ -321,7 +324,7 @@ def _backward(name, maps, a, like, dout, w, out, saved, grads, q_len, kv_len):
     elif dw.shape != w.shape or dw.dtype != w.dtype or dw.device != w.device or not dw.is_contiguous():
         _fail("the learned weights' gradient is %s %s, expected %s %s, contiguous", dw.dtype, tuple(dw.shape), w.dtype, tuple(w.shape))
     a.dw = dw.data_ptr()
-    _enqueue(name, a, like.device, "sgta_attn_bwd_ws_floats", maps, _meta(name, a, maps, (5 * maps, 3)))
+    _enqueue(name, a, like.device, "sgta_attn_bwd_ws_floats", maps, _meta(name, a, maps, backward=True))
     return dq, dk, dv, dw
 
 
