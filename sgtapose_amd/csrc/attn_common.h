@@ -25,7 +25,9 @@ template <int TY> struct El;
 
 // float on the bfloat16 pipe.  A float's 24 significant bits are three bfloat16 numbers, x = hi + mid + lo exactly (each the upper
 // half of what the ones before leave); of the nine products of two such sums the six of at least 2^-16 of the whole are taken, smallest
-// first, each with all its bits into the f32 accumulator: what is left out is below 3 * 2^-24 of |a||b|, the rounding of a few terms.
+// first, each with all its bits into the f32 accumulator.  mid is below 2^-7 of the leading power and lo below 2^-15, so what is left out,
+// mid lo + lo mid + lo lo, is below 2^-21 = 8 * 2^-24 of |a||b| (2 * 2^-24 on average), of the product's sign.  Split to the nearest it
+// would be below 2^-24, but a float next to the largest would become an infinity, and that a not-a-number behind a mask's weight of zero.
 // Six v_mfma_f32_32x32x16_bf16 (192 cycles) in place of eight v_mfma_f32_32x32x2_f32 (512), and the splits, ~44 vector
 // instructions a fragment, overlap them.  Same range as float; what is not finite gives not-a-number in hi - hi: so does x * 0.
 struct Split8 {
