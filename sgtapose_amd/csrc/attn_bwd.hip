@@ -15,7 +15,9 @@
 // run to run and that dQ (f32, Lq x D a head and key block) is never read back.
 //
 // IEEE half: dS is rounded to half as the operand of the next product.  Gradients arrive at any magnitude, so it is first scaled
-// by a power of two that brings the largest |dO| of the row (dQ) or of all queries of the shared heads (dK) next to one.
+// by a power of two that brings the largest |dO| of the row (dQ) or of all queries of the shared heads (dK) next to one.  Values beyond
+// 2^13 / Dv (64 at Dv = 128) could then still take it past the half range, though every operand and result is a half: they take the
+// scale down with them (attn_vmax_kernel finds the largest).
 #include "attn_common.h"
 
 #define DIAG 768               // floats of a wave's 16 x 32 tile in rows of 47, with 15 zeros in front
@@ -27,10 +29,13 @@ __device__ __forceinline__ float pow2_to_one(float top) {          // 2^-exponen
   return (e == 0 || e == 255) ? 1.0f : __uint_as_float((unsigned)(min(max(254 - e, 1), 254)) << 23);
 }
 
+#define VMAX_KEYS 128          // keys of a part at least
 // the workspace, in floats
 struct BwdWork {
   long delta, part, top;       // [maps][B][H][Lq]; per (b, h, query block): sums by bucket, or of d2; largest |dO|
+  long vmax;                   // IEEE half: largest |v| of each part of (b, key / value head)'s keys
   long total;
+  int nv;                      // parts
   int rw, nblk, nsum, nrel;    // attn_dq_kernel's waves by rows and query blocks; floats of a part; distances told apart
   __host__ __device__ BwdWork(const AttnArgs& a, int maps) {
     // (float heads beyond 64: the tiles of two halves leave no room for four waves' sums by distance of a wide table)
@@ -42,9 +47,47 @@ struct BwdWork {
     delta = 0;
     part = (long)maps * a.B * a.H * a.Lq;
     top = part + blocks * nsum;
-    total = top + blocks;
+    vmax = top + blocks;
+    nv = a.dtype == TY_F16 ? (a.Lk + VMAX_KEYS - 1) / VMAX_KEYS : 0;
+    nv = nv > 64 ? 64 : nv;
+    total = vmax + (long)a.B * a.Hkv * nv;
   }
 };
+
+// Parts of the keys of a (b, key / value head): their largest |v|, infinities and not-a-numbers aside.  A launch and one read of v: 4 to 7 us
+// of 77 (32 x 8 heads of 16, 343 tokens, forward and backward) to 424 (4 x 16 heads of 64, 2048).  Looking for the largest dS in the
+// walks, or walking again where a sum is not finite, took 17 to 20 us there, in registers stored.
+__global__ __launch_bounds__(256) void attn_vmax_kernel(AttnArgs a, BwdWork wk) {
+  typedef El<TY_F16>::T T;
+  __shared__ float red[4];
+  const int bh = blockIdx.x / wk.nv, part = blockIdx.x % wk.nv, b = bh / a.Hkv, tid = threadIdx.x, per = a.Dv / 8;
+  const int nk = clamp_len(a.kv_len, b, a.Lk), keys = (nk + wk.nv - 1) / wk.nv, j0 = min(part * keys, nk), n = min(keys, nk - j0);
+  const T* p = (const T*)a.v + b * a.sv[0] + (long)j0 * a.sv[1] + bh % a.Hkv * a.sv[2];
+  float top = 0.0f;
+#pragma unroll 8
+  for (long i = tid; i < (long)n * per; i += 256) {
+    const El<TY_F16>::Raw v = *reinterpret_cast<const El<TY_F16>::Raw*>(p + i / per * a.sv[1] + i % per * 8);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = fabsf((float)v[e]);
+      top = fmaxf(top, x < INFINITY ? x : 0.0f);
+    }
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  if ((tid & 63) == 0) red[tid >> 6] = top;
+  __syncthreads();
+  if (tid == 0) a.ws[wk.vmax + blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+// |P (dO V^T - delta)| is at most 2 Dv |dO| |v|, with lambda for the second map; |dO| is below 2: the power of two that keeps it below 2^15
+__device__ __forceinline__ float value_scale(const AttnArgs& a, const BwdWork& wk, int b, int hk, float lam) {
+  const int lane = threadIdx.x & 63;
+  float top = lane < wk.nv ? a.ws[wk.vmax + (long)(b * a.Hkv + hk) * wk.nv + lane] : 0.0f;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  const float most = top * fmaxf(fabsf(lam), 1.0f) * (float)(4 * a.Dv) * 0x1p-15f;
+  return most > 1.0f ? 0.5f * pow2_to_one(most) : 1.0f;
+}
 
 // LDS of attn_dq_kernel before the bias table: two stages of keys, or what lies over them at the end
 template <int TY, int MAPS, int DQ, int DV, int RW> struct DqLds {
@@ -172,7 +215,7 @@ __global__ __launch_bounds__(256, dq_groups(TY, MAPS, DQ, DV)) void attn_dq_kern
     __syncthreads();
     if (tid == 0) *topw = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   }
-  const float rs = TY == TY_F16 ? pow2_to_one(top) : 1.0f;          // power of two for dS
+  const float rs = TY == TY_F16 ? pow2_to_one(top) * value_scale(a, wk, b, hk, lam) : 1.0f;     // power of two for dS
   const float irs = 1.0f / rs;
 
   const int pos = st + row, pmin = st + row0, pmax = st + row0 + 31;
@@ -524,7 +567,7 @@ __global__ __launch_bounds__(256, (MAPS * DQ + DV > 128 || (TY == TY_F32 && MAPS
     for (int i = lane; i < G * wk.nblk; i += 64) top = fmaxf(top, a.ws[wk.top + ((long)b * a.H + hk * G) * wk.nblk + i]);
 #pragma unroll
     for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-    rs = pow2_to_one(top);
+    rs = pow2_to_one(top) * value_scale(a, wk, b, hk, lam);
   }
   f32x16 dk[MAPS][DQ / 32], dv[DV / 32];
 #pragma unroll
@@ -759,6 +802,10 @@ template <int TY, int MAPS, int DQ, int DV, bool BIAS, int RW> static int launch
 }
 template <int TY, int MAPS, int DQ, int DV, bool BIAS> static int launch_bwd(const AttnArgs* a, hipStream_t stream) {
   const BwdWork wk(*a, MAPS);
+  if (TY == TY_F16) {
+    hipLaunchKernelGGL(attn_vmax_kernel, dim3(a->B * a->Hkv * wk.nv), dim3(256), 0, stream, *a, wk);
+    SGTA_LAUNCH_CHECK();
+  }
   if (int e = wk.rw == 2 ? launch_dq<TY, MAPS, DQ, DV, BIAS, 2>(a, wk, stream) : launch_dq<TY, MAPS, DQ, DV, BIAS, 4>(a, wk, stream)) return e;
   const bool two = row_waves((long)a->B * a->Hkv * cdiv(a->Lk, 128)) == 2;
   if (int e = two ? launch_dkv<TY, MAPS, DQ, DV, BIAS, 2>(a, wk, stream) : launch_dkv<TY, MAPS, DQ, DV, BIAS, 4>(a, wk, stream)) return e;
