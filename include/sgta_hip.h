@@ -509,7 +509,7 @@ int sgta_dcnv2_x3(const float* x, long x_bs, const float* om, long om_bs, const 
  * out2: [B, Lq, H, Dv] contiguous, the second map's product with v (for the backward pass) or NULL.
  * ws: f32 workspace of sgta_attn_fwd_ws_floats() floats (0: not used), written before it is read; calls that may
  * overlap take one each; 16-byte aligned.  Outputs share no memory with each other or with what a call reads.
- * B H ceil(max(Lq, Lk) / 128) is below 2^24, for gradients H num_buckets too. */
+ * scale is from 1e-36 to 1e36.  B H ceil(max(Lq, Lk) / 128) is below 2^24, for gradients H num_buckets too. */
 typedef struct {
   const void *q, *k, *v, *w;
   void *out, *out2;

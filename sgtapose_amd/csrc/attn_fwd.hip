@@ -658,7 +658,7 @@ static int launch_fwd(const AttnArgs* a, hipStream_t stream) {
 int attn_check(const AttnArgs* a, int maps) {
   if (!a || !a->q || !a->k || !a->v || !a->w || !a->out) return SGTA_EBADARG;
   if (a->dtype < 0 || a->dtype > 2 || a->B < 1 || a->Lq < 1 || a->Lk < 1 || a->H < 1 || a->Hkv < 1 || a->H % a->Hkv) return SGTA_EBADARG;
-  if (a->D < 8 || a->D % 8 || a->Dv < 8 || a->Dv % 8 || !(a->scale > 0.0f) || !(a->scale < INFINITY)) return SGTA_EBADARG;
+  if (a->D < 8 || a->D % 8 || a->Dv < 8 || a->Dv % 8 || !(a->scale >= 0.99e-36f) || !(a->scale <= 1.01e36f)) return SGTA_EBADARG;
   if (maps == 1 ? (a->D > 128 || a->Dv != a->D) : (a->D > 64 || a->Dv > 128)) return SGTA_EBADARG;
   if (a->Lq >= 1 << 29 || a->Lk >= 1 << 29 || (long)a->B * a->H * cdiv(a->Lq > a->Lk ? a->Lq : a->Lk, 128) >= MAX_GROUPS) return SGTA_ETOOBIG;
   if (maps == 1 && (!a->lut || a->reach < 1 || a->reach > 1024 || a->num_buckets < 1)) return SGTA_EBADARG;

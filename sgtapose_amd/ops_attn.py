@@ -139,8 +139,8 @@ def _plan(maps, qs, qst, ks, kst, vs, vst, dtype, causal, scale, w_shape, max_di
         _fail("%d sequences of %d, %d with %d heads: B * H * ceil(longest / 128) stays below 2^24", B, Lq, Lk, H)
     if scale is None:
         scale = D ** -0.5
-    if not (scale > 0 and math.isfinite(scale)):
-        _fail("scale %r: a positive number", scale)
+    if not 1e-36 <= scale <= 1e36:
+        _fail("scale %r: a positive number, from 1e-36 to 1e36 (it and its inverse are formed in units of log2)", scale)
     a = _lib.AttnArgs(B=B, Lq=Lq, Lk=Lk, H=H, Hkv=Hkv, D=D, Dv=Dv, causal=int(causal), dtype=DTYPES[dtype], scale=scale)
     size = 4 if dtype == torch.float32 else 2
     _set_strides(a, "sq", _whole("q", qs, qst, size), maps == 2)
@@ -278,7 +278,7 @@ def rel_attention(q, k, v, table, out=None, *, max_distance=128, bidirectional=T
     """softmax(scale q k^T + table[bucket(key - query), head]) v, one pass, nothing of size Lq x Lk in memory.
 
     ``table`` [num_buckets, H] is the learned bias; buckets as ``relative_buckets(num_buckets, max_distance, bidirectional)``.
-    ``scale`` None: D ** -0.5.  ``save``: returns (out, saved) for ``rel_attention_bwd``."""
+    ``scale`` None: D ** -0.5; 1e-36 to 1e36.  ``save``: returns (out, saved) for ``rel_attention_bwd``."""
     _no_graph(save, q, k, v, table)
     a = _operands(1, q, k, v, table, causal, scale, q_len, kv_len, q_start, int(max_distance), bool(bidirectional))
     return _forward("sgta_rel_attn_fwd", 1, a, q, out, q_len, save)
