@@ -217,10 +217,15 @@ template <int TY, int COLS, int ROWS, int NT> struct Dma {
 };
 // The 4 waves of a work-group own 32 rows (queries; keys for dK and dV) each; or two waves share 32 rows, each walking half of the
 // other side, and are joined at the end: twice as many work-groups of half the length, for grids that would leave compute units
-// idle or, ragged or under a causal mask, make the chip wait for the longest.  ``groups``: work-groups of the first kind.
-// Measured, first -> second kind: 640 of them (8 x 8 heads, 1183 ragged, D 64) 33 -> 28 us; 256 (2 x 8 heads, 2048 causal, two maps)
-// forward 93 -> 76, dK dV 122 -> 93, dQ 85 -> 60; 768 (32 x 8 heads, 343) 36 -> 39, 65 -> 71, 52 -> 76.
-__host__ __device__ __forceinline__ int row_waves(long groups) { return groups < 704 ? 2 : 4; }
+// idle or, ragged, make the chip wait for the longest.  ``groups``: work-groups of the first kind; 416 are 1.6 a compute unit.
+// Measured over 343, 1183 and 2048 tokens with and without a causal mask (time of the second kind over the first's, ranges over one and two
+// maps, bfloat16 and float, heads of 32 to 128):                  128        256        384        448        512        640 groups
+//   forward                                                       0.60-0.79  0.69-0.93  0.74-1.06  0.88-1.23  0.90-1.26  0.93-1.18
+//   dQ                                                            0.68-0.85  0.75-1.13  0.79-1.45  0.83-1.77  0.93-1.71  1.01-1.65
+//   dK dV                                                         0.66-0.83  0.73-1.08  0.84-1.20  0.98-1.37  0.99-1.36  0.96-1.26
+// Lengths spread evenly down to a tenth leave half of a forward grid empty: there it crosses at twice as many (640: 0.78-1.07, 960:
+// 0.81-1.16), the gradients at as many (480: 0.83-1.54).
+__host__ __device__ __forceinline__ int row_waves(long groups) { return groups < 416 ? 2 : 4; }
 #define MAX_PITCH (1 << 24)
 #define MAX_GROUPS (1L << 24)  // work-groups of 256 in a launch: a grid's work-items are counted in 32 bits
 // until at most KEEP of this wave's loads are in flight

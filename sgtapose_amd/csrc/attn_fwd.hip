@@ -650,7 +650,8 @@ static int launch_fwd(const AttnArgs* a, hipStream_t stream) {
     }
     return SGTA_OK;
   }
-  return row_waves((long)a->B * a->H * cdiv(a->Lq, 128)) == 2 ? launch_rows<TY, MAPS, DQ, DV, BIAS, 2>(a, tab, stream)
+  const long groups = (long)a->B * a->H * cdiv(a->Lq, 128);
+  return row_waves(a->q_len || a->kv_len ? groups / 2 : groups) == 2 ? launch_rows<TY, MAPS, DQ, DV, BIAS, 2>(a, tab, stream)
                                                               : launch_rows<TY, MAPS, DQ, DV, BIAS, 4>(a, tab, stream);
 }
 

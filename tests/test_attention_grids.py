@@ -1,5 +1,5 @@
-"""The attention kernels' forms for large grids (a wave for every 32 rows, from 704 work-groups of 128 rows on) and the orders in which
-work-groups take heads, at sizes that a 64-bit reference can hold: many heads of short sequences.  Bounds as in test_attention.py.
+"""The attention kernels' forms for large grids (a wave for every 32 rows, from 416 work-groups of 128 rows on, in the forward pass with
+lengths from 832 on) and the orders in which work-groups take heads, at sizes that a 64-bit reference can hold: many heads of short sequences.  Bounds as in test_attention.py.
 
 Work-groups: B H ceil(Lq / 128) forward and for dQ, B Hkv ceil(Lk / 128) for dK and dV.
 """
@@ -11,13 +11,16 @@ from test_attention import ALL, NAMES, Case, check_both, check_forward
 gpu = pytest.mark.gpu
 
 # B, Lq, Lk, H, Hkv: work-groups forward / dK dV, and what B Hkv (B H) is a multiple of
-GRIDS = [(1, 33, 33, 704, 704),        # 704 / 704: the first of the large grids; 8
+GRIDS = [(1, 33, 33, 704, 704),        # 704 / 704; 8
          (2, 130, 140, 176, 176),      # 704 / 704, two blocks a head; 8, lengths that end inside a tile
          (1, 50, 70, 704, 176),        # 704 / 176, shared heads; 8
          (1, 40, 33, 704, 44),         # 704 / 44; heads by 8, key heads not
          (1, 33, 45, 705, 705),        # 705 / 705; neither
-         (1, 36, 35, 703, 703),        # 703 / 703: the last of the small ones
-         (1, 200, 131, 352, 176)]      # 704 / 352, two blocks a head
+         (1, 36, 35, 703, 703),        # 703 / 703; neither
+         (1, 200, 131, 352, 176),      # 704 / 352, two blocks a head
+         (1, 33, 36, 416, 416),        # 416 / 416: the first of the large ones; 8
+         (1, 36, 33, 415, 415),        # 415 / 415: the last of the small ones; neither
+         (2, 130, 40, 208, 208)]       # 832 / 416 with lengths: the first of the large ones of either pass
 EVERY_TYPE = GRIDS[:2]
 
 
@@ -39,7 +42,7 @@ def cases():
 @pytest.mark.parametrize("grid,causal,dtype,n", cases())
 def test_rel_large_grids(grid, causal, dtype, n):
     B, Lq, Lk, H, Hkv = grid
-    for D in {0: (64, 128), 1: (16, 40)}.get(n, ((32, 64, 96, 128, 24)[n - 2],)):
+    for D in {0: (64, 128), 1: (16, 40)}.get(n, ((32, 64, 96, 128, 24, 128, 40, 64)[n - 2],)):
         check_both(Case(1, dtype, B, Lq, Lk, H, Hkv, D, causal=causal, seed=D, **lengths(B, Lq, Lk, causal)))
 
 
@@ -47,7 +50,7 @@ def test_rel_large_grids(grid, causal, dtype, n):
 @pytest.mark.parametrize("grid,causal,dtype,n", cases())
 def test_diff_large_grids(grid, causal, dtype, n):
     B, Lq, Lk, H, Hkv = grid
-    for D, Dv in {0: ((64, 128),), 1: ((32, 64),)}.get(n, (((16, 32), (64, 128), (40, 24), (32, 64), (48, 96))[n - 2],)):
+    for D, Dv in {0: ((64, 128),), 1: ((32, 64),)}.get(n, (((16, 32), (64, 128), (40, 24), (32, 64), (48, 96), (64, 128), (32, 64), (40, 128))[n - 2],)):
         check_both(Case(2, dtype, B, Lq, Lk, H, Hkv, D, Dv, causal=causal, seed=D, **lengths(B, Lq, Lk, causal)))
 
 
