@@ -15,9 +15,9 @@
 // run to run and that dQ (f32, Lq x D a head and key block) is never read back.
 //
 // IEEE half: dS is rounded to half as the operand of the next product.  Gradients arrive at any magnitude, so it is first scaled
-// by a power of two that brings the largest |dO| of the row (dQ) or of all queries of the shared heads (dK) next to one.  Values beyond
-// 2^13 / Dv (64 at Dv = 128) could then still take it past the half range, though every operand and result is a half: they take the
-// scale down with them (attn_vmax_kernel finds the largest).
+// by a power of two that brings the largest |dO| of the row (dQ) or of all queries of the shared heads (dK) next to one.  Values of some
+// thousand could then still take it past the half range, though every operand and result is a half: they take the scale down with them
+// (attn_vmax_kernel finds the largest).
 #include "attn_common.h"
 
 #define DIAG 768               // floats of a wave's 16 x 32 tile in rows of 47, with 15 zeros in front
@@ -32,7 +32,7 @@ __device__ __forceinline__ float pow2_to_one(float top) {          // 2^-exponen
 #define VMAX_KEYS 128          // keys of a part at least
 // the workspace, in floats
 struct BwdWork {
-  long delta, part, top;       // [maps][B][H][Lq]; per (b, h, query block): sums by bucket, or of d2; largest |dO|
+  long delta, part, top;       // [maps][B][H][Lq]; per (b, h, query block): sums by bucket, or of d2; largest |dO|, and sum of a row's
   long vmax;                   // IEEE half: largest |v| of each part of (b, key / value head)'s keys
   long total;
   int nv;                      // parts
@@ -47,7 +47,7 @@ struct BwdWork {
     delta = 0;
     part = (long)maps * a.B * a.H * a.Lq;
     top = part + blocks * nsum;
-    vmax = top + blocks;
+    vmax = top + 2 * blocks;
     nv = a.dtype == TY_F16 ? (a.Lk + VMAX_KEYS - 1) / VMAX_KEYS : 0;
     nv = nv > 64 ? 64 : nv;
     total = vmax + (long)a.B * a.Hkv * nv;
@@ -79,16 +79,16 @@ __global__ __launch_bounds__(256) void attn_vmax_kernel(AttnArgs a, BwdWork wk) 
   __syncthreads();
   if (tid == 0) a.ws[wk.vmax + blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
-// |P (dO V^T - delta)| is at most 2 Dv |dO| |v|, with lambda for the second map; |dO| is below 2: the power of two that keeps it below 2^15
-__device__ __forceinline__ float value_scale(const AttnArgs& a, const BwdWork& wk, int b, int hk, float lam) {
+// X_ij - delta_i = sum_k P_ik (X_ij - X_ik), so |P_ij (X_ij - delta_i)| is at most P (1 - P) 2 max|X| <= sum|dO| max|v| / 2, with lambda for
+// the second map: the power of two that keeps that, for a row's sum ``l1`` already scaled, below 60000 of a half's 65504
+__device__ __forceinline__ float value_scale(const AttnArgs& a, const BwdWork& wk, int b, int hk, float lam, float l1) {
   const int lane = threadIdx.x & 63;
   float top = lane < wk.nv ? a.ws[wk.vmax + (long)(b * a.Hkv + hk) * wk.nv + lane] : 0.0f;
 #pragma unroll
   for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-  const float most = top * fmaxf(fabsf(lam), 1.0f) * (float)(4 * a.Dv) * 0x1p-15f;
+  const float most = top * fmaxf(fabsf(lam), 1.0f) * l1 * (0.5f / 60000.0f);
   return most > 1.0f ? 0.5f * pow2_to_one(most) : 1.0f;
 }
-
 // LDS of attn_dq_kernel before the bias table: two stages of keys, or what lies over them at the end
 template <int TY, int MAPS, int DQ, int DV, int RW> struct DqLds {
   static constexpr int KT = TY == TY_F32 && RW == 4 ? 32 : 64, STAGE = 2 * KT * (MAPS * DQ + DV) * (int)sizeof(typename El<TY>::T);
@@ -117,7 +117,7 @@ __global__ __launch_bounds__(256, dq_groups(TY, MAPS, DQ, DV)) void attn_dq_kern
   extern __shared__ __align__(16) char smem[];       // 2 x (K maps, V) | bias table | 4 waves: sums by distance | 4 waves: DIAG
   const BwdWork wk(a, MAPS);
   float* tab = reinterpret_cast<float*>(smem + DqLds<TY, MAPS, DQ, DV, RW>::ALL);
-  __shared__ float red[4], mend[MAPS][4][32];
+  __shared__ float red[2][4], mend[MAPS][4][32];
   __shared__ double sums[4];
   const int nblk = wk.nblk, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, half = lane >> 5;
   const int bh = blockIdx.x % (a.B * a.H), b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
@@ -125,10 +125,10 @@ __global__ __launch_bounds__(256, dq_groups(TY, MAPS, DQ, DV)) void attn_dq_kern
   const int nq = clamp_len(a.q_len, b, a.Lq), nk = clamp_len(a.kv_len, b, a.Lk), st = start_of(a.q_start, b);
   const int blk0 = blk * 32 * RW, half_of = RW == 2 ? wave >> 1 : 0;         // rows; which half of each tile's keys
   float* part = a.ws + wk.part + ((long)bh * nblk + blk) * wk.nsum;
-  float* topw = a.ws + wk.top + (long)bh * nblk + blk;
+  float* topw = a.ws + wk.top + 2 * ((long)bh * nblk + blk);
   if (blk0 >= nq) {
     for (int i = tid; i < wk.nsum; i += 256) part[i] = 0.0f;
-    if (tid == 0) *topw = 0.0f;
+    if (tid == 0) topw[0] = topw[1] = 0.0f;
     return;
   }
   const int row0 = blk0 + (RW == 2 ? wave & 1 : wave) * 32, row = row0 + li;
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(256, dq_groups(TY, MAPS, DQ, DV)) void attn_dq_kern
   }
   // the row's operands, delta and largest |dO|
   Frag q[MAPS][DQ / 16], g[DV / 16];
-  float m[MAPS], lg[MAPS], dl[MAPS], top = 0.0f;
+  float m[MAPS], lg[MAPS], dl[MAPS], top = 0.0f, l1 = 0.0f;
   // float: every other row's X is computed with its sign turned, so that what is left of the cut-off's mean error cancels in sums over
   // rows (lambda's gradient, the table's)
   const float sx = TY == TY_F32 && (li & 1) ? -1.0f : 1.0f;
@@ -185,6 +185,7 @@ __global__ __launch_bounds__(256, dq_groups(TY, MAPS, DQ, DV)) void attn_dq_kern
       for (int e = 0; e < 8; ++e) {
         s1 = fmaf((float)gr[e], (float)o[e], s1);
         top = fmaxf(top, fabsf((float)gr[e]));
+        if (TY == TY_F16) l1 += fabsf((float)gr[e]);
       }
       if constexpr (MAPS == 2) {
         const typename El<TY>::Raw y = global_raw<TY>(o2 + d, in);
@@ -194,6 +195,7 @@ __global__ __launch_bounds__(256, dq_groups(TY, MAPS, DQ, DV)) void attn_dq_kern
     }
     s1 = half_sum(s1);
     top = half_max(top);
+    if (TY == TY_F16) l1 = half_sum(l1);
     if constexpr (MAPS == 2) {
       s2 = half_sum(s2);
       dl[0] = fmaf(lam, s2, s1);
@@ -208,14 +210,26 @@ __global__ __launch_bounds__(256, dq_groups(TY, MAPS, DQ, DV)) void attn_dq_kern
       lg[p] = ok ? a.stats[2 * at + 1] : INFINITY;
       if (EXACT) lg[p] = exp2_(-lg[p]);
     }
-    float t = top;
+    if constexpr (TY == TY_F16) {
+      float t = top, u = l1;
 #pragma unroll
-    for (int d = 16; d; d >>= 1) t = fmaxf(t, __shfl_xor(t, d));
-    if (lane == 0) red[wave] = t;
-    __syncthreads();
-    if (tid == 0) *topw = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+      for (int d = 16; d; d >>= 1) {
+        t = fmaxf(t, __shfl_xor(t, d));
+        u = fmaxf(u, __shfl_xor(u, d));
+      }
+      if (lane == 0) {
+        red[0][wave] = t;
+        red[1][wave] = u;
+      }
+      __syncthreads();
+      if (tid < 2) topw[tid] = fmaxf(fmaxf(red[tid][0], red[tid][1]), fmaxf(red[tid][2], red[tid][3]));
+    }
   }
-  const float rs = TY == TY_F16 ? pow2_to_one(top) * value_scale(a, wk, b, hk, lam) : 1.0f;     // power of two for dS
+  float rs = 1.0f;                                    // power of two for dS
+  if constexpr (TY == TY_F16) {
+    rs = pow2_to_one(top);
+    rs *= value_scale(a, wk, b, hk, lam, l1 * rs);
+  }
   const float irs = 1.0f / rs;
 
   const int pos = st + row, pmin = st + row0, pmax = st + row0 + 31;
@@ -563,11 +577,19 @@ __global__ __launch_bounds__(256, (MAPS * DQ + DV > 128 || (TY == TY_F32 && MAPS
   }
   float rs = 1.0f;
   if constexpr (TY == TY_F16) {
-    float top = 0.0f;
-    for (int i = lane; i < G * wk.nblk; i += 64) top = fmaxf(top, a.ws[wk.top + ((long)b * a.H + hk * G) * wk.nblk + i]);
+    float top = 0.0f, l1 = 0.0f;
+    for (int i = lane; i < G * wk.nblk; i += 64) {
+      const float* t = a.ws + wk.top + 2 * (((long)b * a.H + hk * G) * wk.nblk + i);
+      top = fmaxf(top, t[0]);
+      l1 = fmaxf(l1, t[1]);
+    }
 #pragma unroll
-    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-    rs = pow2_to_one(top) * value_scale(a, wk, b, hk, lam);
+    for (int d = 32; d; d >>= 1) {
+      top = fmaxf(top, __shfl_xor(top, d));
+      l1 = fmaxf(l1, __shfl_xor(l1, d));
+    }
+    rs = pow2_to_one(top);
+    rs *= value_scale(a, wk, b, hk, lam, l1 * rs);
   }
   f32x16 dk[MAPS][DQ / 32], dv[DV / 32];
 #pragma unroll

@@ -43,3 +43,14 @@ def test_few_large_values(maps):
         c.v[:, 70] = 3e4 * c.v[:, 70].sign()
         c.v[:, 3] = -2e4 * c.v[:, 3].sign()
         check_both(c)
+
+
+@gpu
+@pytest.mark.parametrize("Lq,Lk,Hkv,D", [(8, 130, 2, 64), (1, 63, 8, 24), (64, 200, 2, 96)])
+def test_small_weights_beside_large_values(Lq, Lk, Hkv, D):
+    """Values of some thousand alone leave the scale where it is: keys of small weights keep what |dO| next to one gives them."""
+    for seed in range(4):
+        c = Case(1, torch.float16, 2, Lq, Lk, 4 if Hkv == 2 else 8, Hkv, D, buckets=16, far=40, seed=seed)
+        c.w = (c.w.float() * 30).half()
+        c.v = (c.v.float() * 3000).half()
+        check_both(c)
