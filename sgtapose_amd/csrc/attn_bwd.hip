@@ -5,6 +5,10 @@
 // Two maps share X:  dS1 = P1 o (X - d1), dS2 = -lambda P2 o (X - d2), d_p = rowsum(dO o O_p), dV = (P1 - lambda P2)^T dO,
 //   dlambda = - sum of d2.
 //
+// Held in fewer bits than f32, in 16-bit calls: P and dS, rounded to the element type as operands of the products that give dV, dQ and dK
+// (all of which sum in f32), and delta, from the rounded output (mended below).  dQ, dK and dV of bfloat16 are 2.4e-3 off, 1.7e-3 by
+// their own rounding alone; a second operand for the rest would add a product to each of the three.
+//
 // No atomics and no Lq x Lk array: every sum has one owner and a fixed order.
 //   attn_dq_kernel   a wave owns 32 queries and walks the keys: delta, dQ, the table's gradient by distance
 //                    (4 x 16 heads of 64, 2048 tokens, bfloat16: 165 us, vector pipe 54 % of the cycles, matrix 29, LDS 30)
