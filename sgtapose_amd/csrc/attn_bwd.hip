@@ -11,9 +11,9 @@
 //
 // No atomics and no Lq x Lk array: every sum has one owner and a fixed order.
 //   attn_dq_kernel   a wave owns 32 queries and walks the keys: delta, dQ, the table's gradient by distance
-//                    (4 x 16 heads of 64, 2048 tokens, bfloat16: 165 us, vector pipe 54 % of the cycles, matrix 29, LDS 30)
+//                    (4 x 16 heads of 64, 2048 tokens, bfloat16: 165 us, vector pipe 55 % of the cycles, matrix 30, LDS 30)
 //   attn_dkv_kernel  a wave owns 32 keys and walks the queries of all heads that share them: dK, dV
-//                    (the same: 186 us, matrix 35, vector 36, LDS 37; heads beyond 64: one work-group on a CU, by registers)
+//                    (the same: 187 us, matrix 35, vector 37, LDS 37; heads beyond 64: one work-group on a CU, by registers)
 //   *_dw_kernel      sums the work-groups' parts of the learned weights' gradient
 // The price is that scores and X are computed twice (7 products instead of 5); what it buys is that gradients are the same from
 // run to run and that dQ (f32, Lq x D a head and key block) is never read back.
@@ -102,6 +102,8 @@ template <int TY, int MAPS, int DQ, int DV, int RW> struct DqLds {
 };
 // Work-groups on a CU that the registers are held to.  float heads of 32: three, at the price of a few registers stored outside the
 // loop (32 x 8 heads, 343 tokens: 52 us where two take 67); 16-bit heads up to 64: three (4 x 16 heads, 2048 tokens: 165 us, two 188).
+// Two for float heads of 64 (11 registers stored where two waves share rows) and float two-map heads of 32: there 38 are, 14 of them read
+// back in the loop, and 15 in the form for large grids (2 x 777 tokens, 8 heads: 68 us, most of it one wave's latency).
 constexpr int dq_groups(int ty, int maps, int dq, int dv) {
   return ty == TY_F32 ? (dq * maps + dv > 128 ? 1 : maps > 1 || dq > 32 ? 2 : 3) : maps > 1 || dq > 64 ? 2 : dq > 32 ? 3 : 4;
 }
@@ -499,6 +501,8 @@ __global__ __launch_bounds__(256, dq_groups(TY, MAPS, DQ, DV)) void attn_dq_kern
   }
 }
 
+// All 512 registers of a SIMD where heads are large (floats from 64, 16-bit two-map ones of 64 / 128): one work-group on a compute unit.
+// Float two-map heads of 64 / 128 still store 21 and read 23 back in the loop, float heads of 128 on large grids 16.
 template <int TY, int MAPS, int DQ, int DV, bool BIAS, int RW>
 __global__ __launch_bounds__(256, (MAPS * DQ + DV > 128 || (TY == TY_F32 && MAPS * DQ + DV > 64)) ? 1 : 2) void attn_dkv_kernel(AttnArgs a, int nblk) {
   typedef typename El<TY>::T T;

@@ -7,16 +7,17 @@
 // attn_fwd_kernel: 4 waves of 32 queries share 64-key tiles of K and V in LDS (double buffered, the next tile's copies in flight
 //   over the present one's products).  S^T = K Q^T puts the query on the lane: row statistics are in-lane but for one lane-half
 //   exchange, and the weights are the next product's operand as they stand: O^T += V^T P^T.
-//   Heads of 64 (4 x 16 heads, 2048 tokens, bfloat16): 105 us = 650 TFLOP/s, bound by the vector pipe (57 % of the cycles: exponentials,
-//   bias, maximum; matrix pipe 30); heads of 128 (16 heads, 8192 causal, half): 320 us = 860, matrix 40, vector 42, LDS 41 %.
+//   Heads of 64 (4 x 16 heads, 2048 tokens, bfloat16): 106 us = 650 TFLOP/s, bound by the vector pipe (57 % of the cycles: exponentials,
+//   bias, maximum; matrix pipe 29); heads of 128 (16 heads, 8192 causal, half): 315 us = 870 with pauses between the calls (385 back to
+//   back, at the power limit), matrix 40, vector 42, LDS 41 %.
 //   Held in fewer bits than f32, in 16-bit calls: a weight, rounded to the element type as the product's operand (their sum is not).  An
 //   output of bfloat16 is 2.1e-3 to 2.6e-3 off with it, 1.7e-3 by its own rounding alone.  The rounding's rest as a second operand took
 //   two maps' forward pass from 66 to 80 us (2 x 8 heads of 64 / 128, 2048 causal), their single-token case from 21.7 to 22.9.
 // attn_step_kernel: few queries (at most 32 rows of all the heads that share a key / value head): these rows are one tile, the
 //   keys are split over the grid and over the 4 waves, each with a private LDS tile and no barrier in the loop; the parts are
 //   joined in LDS and, where the grid splits, by attn_join_kernel.
-//   16 x 1 tokens against 37 MB of ragged caches: 12.6 us, of which a call of one tile takes 6.4 (launch, lengths, a tile's latency,
-//   the join in LDS), and 3.8 for the parts' join.
+//   16 x 1 tokens against 37 MB of ragged caches: 13 us, of which a call of one tile takes 6.4 to 7 (launch, lengths, a tile's latency,
+//   the join in LDS), and 4 for the parts' join.
 #include "attn_common.h"
 
 // One wave's 32 query rows: fragments, running statistics, the accumulated O^T.
@@ -181,7 +182,8 @@ template <int TY, int MAPS, int DQ, int DV, bool BIAS> struct FwdWave {
 
 // The work-group's place: b, key / value head, query head and query block.  Heads that share K and V run on one XCD where the head
 // count allows it (work-groups b and b + 8 share one).  Without a causal mask an XCD takes one head after the other; under one the
-// longest rows of all heads come first (2 x 8 heads, 2048 tokens, two maps: 65 us, head by head 74; 16 heads, 8192 tokens: 364, 374).
+// longest rows of all heads come first (2 x 8 heads, 2048 tokens, two maps: 65 us, head by head 74; 16 heads, 8192 tokens, back to back:
+// 364, 374).
 struct FwdPlace { int b, h, blk; bool ok; };
 __device__ __forceinline__ FwdPlace fwd_place(const AttnArgs& a, int nblk) {
   FwdPlace w;

@@ -454,7 +454,8 @@ struct FinishOne {
 
 // Few tokens: the weights are read once, straight into registers.  A work-group has 16 channels and up to 16 MT tokens
 // (blockIdx.y: the next 16 MT); its 16 waves share k in pieces of 64 bytes and are summed in LDS.  4 x 4096 x 4096: 6.4 us for 17 MB,
-// most of it the latency of launch, one round of loads and the sum.
+// most of it the latency of launch, one round of loads and the sum.  (33 to 64 tokens at any alignment: 1024 threads leave 128 registers
+// each, and 44 are stored in the loop.)
 template <int MT, bool RAGGED>
 __global__ __launch_bounds__(1024) void linear_i8_few_kernel(I8Args a) {
   __shared__ i32x4 part[16][MT][64];
