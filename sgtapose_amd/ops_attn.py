@@ -13,8 +13,9 @@ Lengths: ``kv_len`` / ``q_len`` int32 [B] on the GPU (None: all).  What lies beh
 the first query among the keys (None: 0); a new token against a cache that already holds it has q_start = kv_len - 1.
 ``causal``: a query at position p sees keys j <= p.  A query that sees no key has an output and gradients of zero.
 
-Table values of any size: -inf hides a bucket's keys, and finite ones keep the scores' accuracy up to 1.4e9 in magnitude (2^31 in units of
-log2); beyond, down to a type's lowest value, they absorb the scores, so that a query that only such keys are left for weighs them evenly.
+Table values of any size: -inf hides a bucket's keys; finite ones keep the scores' accuracy up to 7e8 in magnitude (2^30 in units of log2)
+and, up to twice that, the accuracy of scores below 40 (a mask of -1e9).  Beyond, down to a type's lowest value, they absorb the scores,
+so that a query that only such keys are left for weighs them evenly.
 
 Within the lengths a value that is not finite may also reach positions from which the mask hides it (0 times infinity), as in the
 plain products.  float32 operands are split into three bfloat16 numbers, so that an infinity among them gives not-a-numbers.
